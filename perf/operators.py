@@ -281,7 +281,7 @@ def _plain_prompt(s):
     keep = (i[None, :, None] >= i[None, None, :]) & (token < t)[:, :, None]
     scores = _beaver(qc, rqc, kc.transpose(3, 4), rkc.transpose(3, 4), party, bw)[:, :, keep]
     states = _beaver(kd.transpose(3, 4), rkd.transpose(3, 4), vc, rvc, party, bw)
-    out1 = torch.cat((scores.reshape(-1), states.reshape(-1))) + s["z1"]
+    out1 = torch.cat((scores.reshape(-1), states.permute(2, 0, 1, 3, 4).reshape(-1))) + s["z1"]
 
     nt = b * h * _tri(c)
     gap = (i[:, None] - i[None, :]).clamp(min=0, max=t)
@@ -290,15 +290,15 @@ def _plain_prompt(s):
     ends = torch.tensor([e for _, e in _chunks(c)], device="cuda")
     between = ends[:, None] - ends[None, :]
     coef = torch.where(between >= 0, pw[:, between.clamp(min=0)], 0)  # (h, nc, nc)
-    ds = s["pds"][nt:].reshape(b, h, nc, dk * dv)
+    ds = s["pds"][nt:].reshape(nc, b, h, dk * dv).permute(1, 2, 0, 3)
     s0 = s["s0"].reshape(b, h, 1, dk * dv).to(torch.int64)
     carried = _mm(coef, ds, bw) + pw[:, ends][..., None] * s0
-    out2 = torch.cat((pd.reshape(-1), carried.reshape(-1)))
+    out2 = torch.cat((pd.reshape(-1), carried.permute(2, 0, 1, 3).reshape(-1)))
 
     full, rfull = (torch.zeros(b, h, nc, CHUNK, CHUNK, dtype=torch.int64, device="cuda") for _ in range(2))
     full[:, :, keep] = s["ps"][:nt].reshape(b, h, -1).to(torch.int64)
     rfull[:, :, keep] = s["ps_ms"][:nt].reshape(b, h, -1).to(torch.int64)
-    st, rst = (torch.cat((a.reshape(b, h, 1, dk, dv), y[nt:].reshape(b, h, nc, dk, dv)[:, :, :-1]), dim=2)
+    st, rst = (torch.cat((a[None], y[nt:].reshape(nc, b, h, dk, dv)[:-1])).permute(1, 2, 0, 3, 4)
                for a, y in ((s["s0"], s["ps"]), (s["s0_ms"], s["ps_ms"])))
     o = _beaver(full, rfull, vc, rvc, party, bw) + _beaver(qd, rqd, st, rst, party, bw)
     o = o.reshape(b, h, nc * CHUNK, dv)[:, :, :t].transpose(1, 2).reshape(-1)
@@ -353,7 +353,7 @@ def exact(case, seed):
     nd, nt = b * h * t * dk, b * h * _tri(c)
     qd, kd, rqd, rkd = (wide[i][a * nd:(a + 1) * nd].reshape(b, h, t, dk) for i in ("qkd", "qkd_ms") for a in (0, 1))
     pds_p, ps_p, ps_pm = (wide[i][:nt].reshape(b, h, -1) for i in ("pds", "ps", "ps_ms"))
-    pds_s, ps_s, ps_sm = (wide[i][nt:].reshape(b, h, -1, dk, dv) for i in ("pds", "ps", "ps_ms"))
+    pds_s, ps_s, ps_sm = (wide[i][nt:].reshape(-1, b, h, dk, dv) for i in ("pds", "ps", "ps_ms"))
     dq, dk_, sc, ss, dec, car, outs, pos = [], [], [], [], [], [], [], 0
     run_coef = []
     for n, (a, e) in enumerate(_chunks(c)):
@@ -369,17 +369,17 @@ def exact(case, seed):
         total = pw[:, e].reshape(1, h, 1, 1) * s0
         run_coef.append(e)
         for j, end in enumerate(run_coef):
-            total = total + pw[:, e - end].reshape(1, h, 1, 1) * pds_s[:, :, j]
+            total = total + pw[:, e - end].reshape(1, h, 1, 1) * pds_s[j]
         car.append(total)
         full, rfull = (torch.zeros(b, h, m, m, dtype=torch.int64, device="cuda") for _ in range(2))
         full[:, :, low[0], low[1]] = ps_p[:, :, pos:pos + size]
         rfull[:, :, low[0], low[1]] = ps_pm[:, :, pos:pos + size]
-        before, rbefore = (s0, rs0) if n == 0 else (ps_s[:, :, n - 1], ps_sm[:, :, n - 1])
+        before, rbefore = (s0, rs0) if n == 0 else (ps_s[n - 1], ps_sm[n - 1])
         outs.append(_share(full, rfull, tr(v[:, :, a:e]), tr(rv[:, :, a:e]), p)
                     + _share(qd[:, :, a:e], rqd[:, :, a:e], tr(before), tr(rbefore), p))
         pos += size
     flat = lambda x, d: torch.cat(x, dim=d).reshape(-1)  # noqa: E731
-    stack = lambda x: torch.stack(x, dim=2).reshape(-1)  # noqa: E731
+    stack = lambda x: torch.stack(x).reshape(-1)  # noqa: E731
     out0 = torch.cat((flat(dq, 2), flat(dk_, 2)))
     out1 = torch.cat((flat(sc, 2), stack(ss))) + wide["z1"]
     out2 = torch.cat((flat(dec, 2), stack(car)))
