@@ -55,6 +55,16 @@ class MaskWire(ctypes.Structure):
     _fields_ = [("d_mask", _vp), ("n", _u64), ("d_share0", _vp), ("d_share1", _vp)]
 
 
+class Q4Weights(ctypes.Structure):
+    """ddg_q4_weights: public 4-bit weights of a (K x N) layer, device pointers."""
+    _fields_ = [("K", _i32), ("N", _i32), ("group", _i32), ("d_q", _vp), ("d_step", _vp), ("d_bias2s", _vp)]
+
+
+class LinattnShape(ctypes.Structure):
+    """ddg_linattn_shape."""
+    _fields_ = [(n, _i32) for n in ("batch", "heads", "tokens", "dk", "dv", "chunk", "pow_n")]
+
+
 # int exchange(void *user, int party, const void *d_send, void *d_recv, uint64_t bytes, void *stream)
 COMM_EXCHANGE = ctypes.CFUNCTYPE(_i32, _vp, _i32, _vp, _vp, _u64, _vp)
 
@@ -64,8 +74,9 @@ class Comm(ctypes.Structure):
     _fields_ = [("user", _vp), ("exchange", COMM_EXCHANGE)]
 
 
-ACT_NONE, ACT_RELU, ACT_TRUNC = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_TRUNC, ACT_FLOOR = 0, 1, 2, 3
 _C, _W, _M = ctypes.POINTER(Cursor), ctypes.POINTER(Wire), ctypes.POINTER(MaskWire)
+_Q4, _LA, _i64 = ctypes.POINTER(Q4Weights), ctypes.POINTER(LinattnShape), ctypes.c_int64
 
 # name -> (restype, argtypes); kept in the order of include/ddg_fss.h
 SIGNATURES = {
@@ -153,6 +164,26 @@ SIGNATURES = {
     "ddg_op_fc_keygen": (_i32, [_vp, _C, _i32, _i32, _i32, _M, _M]),
     "ddg_op_concat_protein_keygen": (_i32, [_vp, _C, _i32, _M, _M]),
     "ddg_op_output_keygen": (_i32, [_vp, _C, _M]),
+    "ddg_q4_row_bytes": (_u64, [_i32]),
+    "ddg_q4_quantize": (_i32, [_i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "ddg_fc_q4_share": (_i32, [_i32, _i32, _i32, _Q4, _vp, _i64, _vp, _vp, _vp]),
+    "ddg_decay_table": (_i32, [_i32, _i32, _i32, _i32, ctypes.POINTER(ctypes.c_double), _vp]),
+    "ddg_linattn_sizes": (_i32, [_LA, ctypes.POINTER(_i64)]),
+    "ddg_linattn_decay": (_i32, [_i32, _LA, _i64, _vp, _vp, _vp, _vp]),
+    "ddg_linattn_carry": (_i32, [_i32, _LA, _vp, _vp, _vp, _vp, _vp]),
+    "ddg_linattn_chunk_share": (_i32, [_i32, _i32, _LA, _i64] + [_vp] * 7),
+    "ddg_linattn_output_share": (_i32, [_i32, _i32, _LA, _i64] + [_vp] * 11),
+    "ddg_linattn_step_share": (_i32, [_i32, _i32, _LA, _i64] + [_vp] * 8),
+    "ddg_linattn_step_output_share": (_i32, [_i32, _i32, _LA, _i64] + [_vp] * 8),
+    "ddg_op_fc_q4_key_bytes": (_u64, [_i32] * 6),
+    "ddg_op_fc_q4_keygen": (_i32, [_vp, _C, _Q4, _i32, _i32, _M, _M]),
+    "ddg_op_fc_q4_eval": (_i32, [_vp, _C, _Q4, _i32, _i32, _W, _W]),
+    "ddg_linattn_key_bytes": (_u64, [_i32, _i32, _LA, _i32]),
+    "ddg_linattn_keygen": (_i32, [_vp, _C, _LA, _vp, _M, _M, _M, _M]),
+    "ddg_linattn_eval": (_i32, [_vp, _C, _LA, _vp, _W, _W, _W, _W]),
+    "ddg_linattn_step_key_bytes": (_u64, [_i32, _i32, _LA]),
+    "ddg_linattn_step_keygen": (_i32, [_vp, _C, _LA, _vp, _M, _M, _M, _M]),
+    "ddg_linattn_step_eval": (_i32, [_vp, _C, _LA, _vp, _W, _W, _W, _W]),
     "ddg_launch_count": (_u64, []),
     "ddg_key_chunk_bytes": (_u64, [_i32, _i32, _i32]),
     "ddg_key_checksum": (_i32, [_vp, _u64, ctypes.POINTER(_u64), _vp]),
@@ -247,6 +278,63 @@ def gate_round2(kind, bw, scale, n, party, d_xhat, d_hi_own, d_hi_peer, d_lo_own
                 stream=None):
     check(lib().ddg_gate_round2(kind, bw, scale, n, party, d_xhat, d_hi_own, d_hi_peer, d_lo_own, d_lo_peer, d_key,
                                 d_share, stream))
+
+
+# ---------------------------------------------------------------- secure token model (share level)
+
+def q4_quantize(K, N, group, d_w, d_q, d_step, stream=None):
+    """4-bit codes and steps of an int64 device matrix (K x N); see ddg_q4_quantize."""
+    check(lib().ddg_q4_quantize(K, N, group, d_w, d_q, d_step, stream))
+
+
+def fc_q4_share(bw, party, M, w: Q4Weights, d_xhat, ldx, d_c, d_out, stream=None):
+    """One party's share of a layer with 4-bit public weights; see ddg_fc_q4_share."""
+    check(lib().ddg_fc_q4_share(bw, party, M, w, d_xhat, ldx, d_c, d_out, stream))
+
+
+def decay_table(bw, scale, lambdas, n):
+    """(heads, n + 1) ring elements lambda^i at the scale (numpy); see ddg_decay_table."""
+    import numpy as np
+
+    lam = np.ascontiguousarray(lambdas, dtype=np.float64)
+    out = np.zeros((lam.size, n + 1), dtype=np.uint32 if bw == 32 else np.uint64)
+    check(lib().ddg_decay_table(bw, scale, lam.size, n, lam.ctypes.data_as(ctypes.POINTER(ctypes.c_double)),
+                                out.ctypes.data))
+    return out
+
+
+def linattn_sizes(shape: LinattnShape) -> dict:
+    """Ring elements of the arrays of one linear attention call; see ddg_linattn_sizes."""
+    out = (_i64 * 6)()
+    check(lib().ddg_linattn_sizes(shape, out))
+    return dict(zip(("qkv", "qkd", "ps", "state", "step", "out"), [int(v) for v in out]))
+
+
+def linattn_decay(bw, shape, ld, d_pow, d_qkv, d_out, stream=None):
+    check(lib().ddg_linattn_decay(bw, shape, ld, d_pow, d_qkv, d_out, stream))
+
+
+def linattn_carry(bw, shape, d_pow, d_ps, d_s0, d_out, stream=None):
+    check(lib().ddg_linattn_carry(bw, shape, d_pow, d_ps, d_s0, d_out, stream))
+
+
+def linattn_chunk_share(bw, party, shape, ld, d_qkv, d_qkv_ms, d_kd, d_kd_ms, d_z, d_out, stream=None):
+    check(lib().ddg_linattn_chunk_share(bw, party, shape, ld, d_qkv, d_qkv_ms, d_kd, d_kd_ms, d_z, d_out, stream))
+
+
+def linattn_output_share(bw, party, shape, ld, d_qkv, d_qkv_ms, d_qd, d_qd_ms, d_ps, d_ps_ms, d_s0, d_s0_ms, d_z,
+                         d_out, stream=None):
+    check(lib().ddg_linattn_output_share(bw, party, shape, ld, d_qkv, d_qkv_ms, d_qd, d_qd_ms, d_ps, d_ps_ms, d_s0,
+                                         d_s0_ms, d_z, d_out, stream))
+
+
+def linattn_step_share(bw, party, shape, ld, d_pow, d_qkv, d_qkv_ms, d_s, d_s_ms, d_z, d_out, stream=None):
+    check(lib().ddg_linattn_step_share(bw, party, shape, ld, d_pow, d_qkv, d_qkv_ms, d_s, d_s_ms, d_z, d_out, stream))
+
+
+def linattn_step_output_share(bw, party, shape, ld, d_pow, d_qkv, d_qkv_ms, d_yw, d_yw_ms, d_z, d_out, stream=None):
+    check(lib().ddg_linattn_step_output_share(bw, party, shape, ld, d_pow, d_qkv, d_qkv_ms, d_yw, d_yw_ms, d_z,
+                                              d_out, stream))
 
 
 # ---------------------------------------------------------------- parties

@@ -80,6 +80,22 @@ int ew_sub(T *out, const T *a, const T *b, uint64_t n, cudaStream_t st)
     return DDG_OK;
 }
 
+template <typename T>
+__global__ void k_offset(T *out, const T *a, T c, uint64_t n)
+{
+    GRID_STRIDE(i, n) out[i] = a[i] + c;
+}
+
+template <typename T>
+int ew_offset(T *out, const T *a, T c, uint64_t n, cudaStream_t st)
+{
+    if (!n) return DDG_OK;
+    k_offset<T><<<ew_grid(n), 256, 0, st>>>(out, a, c, n);
+    note_launch();
+    DDG_CUDA(cudaGetLastError());
+    return DDG_OK;
+}
+
 __device__ __forceinline__ uint64_t bc_index(uint64_t e, int bc, int R, int C)
 {
     if (bc == BC_ROW) return e / uint64_t(C);                                   // (b*R + i)
@@ -423,6 +439,7 @@ int split_shares(const T *v, uint64_t n, const AesKey &dk, uint32_t op, uint32_t
 #define INST(T)                                                                                                  \
     template int ew_add<T>(T *, const T *, const T *, uint64_t, cudaStream_t);                                   \
     template int ew_sub<T>(T *, const T *, const T *, uint64_t, cudaStream_t);                                   \
+    template int ew_offset<T>(T *, const T *, T, uint64_t, cudaStream_t);                                        \
     template int beaver_ew<T>(int, const EwShape &, Bcast, const T *, const T *, const T *, const T *, const T *, \
                               T *, cudaStream_t, const T *, const T *);                                                                \
     template int beaver_ew_z<T>(const EwShape &, Bcast, const T *, const T *, const T *, T *, cudaStream_t);     \

@@ -19,6 +19,7 @@
 #include "gates.cuh"
 #include "linear.cuh"
 #include "ot.cuh"
+#include "token.cuh"
 
 namespace ddg {
 
@@ -33,6 +34,26 @@ struct Tn {
     uint64_t n = 0;
     const T *ms0 = nullptr;  // eval: own mask share; dealer: party 0's
     const T *ms1 = nullptr;  // dealer: party 1's
+};
+
+// elements [at, at + n) of a tensor
+template <typename T>
+Tn<T> slice(const Tn<T> &t, uint64_t at, uint64_t n)
+{
+    Tn<T> r;
+    r.n = n;
+    if (t.v) r.v = t.v + at;
+    if (t.v2) r.v2 = t.v2 + at;
+    if (t.ms0) r.ms0 = t.ms0 + at;
+    if (t.ms1) r.ms1 = t.ms1 + at;
+    return r;
+}
+
+// a layer's 4-bit weights with its bias << s
+template <typename T>
+struct Q4Layer {
+    Q4 w;
+    const T *b2s = nullptr;
 };
 
 // ------------------------------------------------------------------ executors
@@ -125,6 +146,25 @@ struct SizeExec : ExecBase<T> {
     }
     Tn<T> concat(const Tn<T> &a, const Tn<T> &b) { return mk(a.n + b.n); }
     void output(const Tn<T> &o) { take(words(o.n)); }
+    Tn<T> product(uint64_t n) { take(words(n)); return mk(n); }
+    Tn<T> fc_q4(const Tn<T> &, const Q4Layer<T> &w, int M) { return product(uint64_t(M) * w.w.N); }
+    Tn<T> floor_in(const Tn<T> &x) { return x; }
+    void floor_out(Tn<T> &) {}
+    Tn<T> la_decay(const LaShape &s, const T *, const Tn<T> &) { return mk(2 * s.n_decayed()); }
+    Tn<T> la_chunk(const LaShape &s, Tn<T> &x, Tn<T> &qk) { ensure_ms(x), ensure_ms(qk); return product(s.n_ps()); }
+    Tn<T> la_carry(const LaShape &s, const T *, const Tn<T> &, const Tn<T> *) { return mk(s.n_ps()); }
+    Tn<T> la_output(const LaShape &s, Tn<T> &, Tn<T> &, Tn<T> &ps, Tn<T> *s0)
+    {
+        ensure_ms(ps);
+        if (s0) ensure_ms(*s0);
+        return product(s.n_out());
+    }
+    Tn<T> la_step(const LaShape &s, const T *, Tn<T> &x, Tn<T> &S) { ensure_ms(x), ensure_ms(S); return product(s.n_step()); }
+    Tn<T> la_step_output(const LaShape &s, const T *, Tn<T> &, Tn<T> &syw)
+    {
+        ensure_ms(syw);
+        return product(s.bh() * s.dv);
+    }
 };
 
 // ---- dealer (GPU): the masks travel through the graph like values do
@@ -284,6 +324,96 @@ struct DealerExec : ExecBase<T> {
         t.v = alloc(t.n);
         if (this->err == DDG_OK) ok(concat_rows<T>(a.v, b.v, t.v, this->B, PROT, PROT, this->st));
         return t;
+    }
+    // a product's dealer word: `word` writes (product of the masks + output mask) into Z
+    template <class F>
+    Tn<T> product(uint64_t n, F &&word)
+    {
+        Tn<T> t;
+        t.n = n;
+        t.v = rand(n);
+        T *Z = alloc(n);
+        if (this->err == DDG_OK) ok(word(t.v, Z));
+        share_section(Z, n, nullptr, nullptr);
+        return t;
+    }
+    Tn<T> fc_q4(const Tn<T> &x, const Q4Layer<T> &w, int M)
+    {
+        return product(uint64_t(M) * w.w.N, [&](const T *rout, T *Z) {
+            Q4Args<T> a;  // r_y - r_x . W
+            a.w = w.w, a.M = M, a.x = x.v, a.ldx = w.w.K, a.sign = T(0) - T(1), a.Add = rout, a.out = Z;
+            return ::ddg::fc_q4<T>(a, this->st);
+        });
+    }
+    // The non-negative truncation gate as a signed floor: with o = 2^(bw-2),
+    // x_hat = (x + o) + (r - o), and floor((x + o) / 2^s) + r_out =
+    // floor(x / 2^s) + (r_out + 2^(bw-2-s)), so only the dealer's masks move.
+    Tn<T> floor_in(const Tn<T> &x)
+    {
+        Tn<T> t;
+        t.n = x.n;
+        t.v = alloc(x.n);
+        if (this->err == DDG_OK) ok(ew_offset<T>(t.v, x.v, T(0) - (T(1) << (this->bw - 2)), x.n, this->st));
+        return t;
+    }
+    void floor_out(Tn<T> &y)
+    {
+        if (this->err == DDG_OK) ok(ew_offset<T>(y.v, y.v, T(1) << (this->bw - 2 - this->s), y.n, this->st));
+    }
+    Tn<T> la_decay(const LaShape &s, const T *pow, const Tn<T> &x)
+    {
+        Tn<T> t;
+        t.n = 2 * s.n_decayed();
+        t.v = alloc(t.n);
+        if (this->err == DDG_OK) ok(::ddg::la_decay<T>(s, s.width(), pow, x.v, t.v, this->st));
+        return t;
+    }
+    Tn<T> la_chunk(const LaShape &s, Tn<T> &x, Tn<T> &qk)
+    {
+        ensure_ms(x), ensure_ms(qk);
+        return product(s.n_ps(), [&](const T *rout, T *Z) {
+            LaChunkArgs<T> a;
+            a.ld = s.width(), a.qkv = x.v, a.kd = qk.v + s.n_decayed(), a.z = rout, a.out = Z;
+            return ::ddg::la_chunk<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_carry(const LaShape &s, const T *pow, const Tn<T> &ps, const Tn<T> *s0)
+    {
+        Tn<T> t;
+        t.n = s.n_ps();
+        t.v = alloc(t.n);
+        if (this->err == DDG_OK) ok(::ddg::la_carry<T>(s, pow, ps.v, s0 ? s0->v : nullptr, t.v, this->st));
+        return t;
+    }
+    Tn<T> la_output(const LaShape &s, Tn<T> &x, Tn<T> &qk, Tn<T> &ps, Tn<T> *s0)
+    {
+        ensure_ms(ps);
+        if (s0) ensure_ms(*s0);
+        return product(s.n_out(), [&](const T *rout, T *Z) {
+            LaOutArgs<T> a;
+            a.ld = s.width(), a.qkv = x.v, a.qd = qk.v, a.ps = ps.v, a.s0 = s0 ? s0->v : nullptr;
+            a.z = rout, a.out = Z;
+            return ::ddg::la_output<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_step(const LaShape &s, const T *pow, Tn<T> &x, Tn<T> &S)
+    {
+        ensure_ms(x), ensure_ms(S);
+        return product(s.n_step(), [&](const T *rout, T *Z) {
+            LaStepArgs<T> a;
+            a.ld = s.width(), a.pow = pow, a.qkv = x.v, a.s = S.v, a.z = rout, a.out = Z, a.lam = T(0) - T(1);
+            return ::ddg::la_step<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_step_output(const LaShape &s, const T *pow, Tn<T> &x, Tn<T> &syw)
+    {
+        ensure_ms(syw);
+        return product(s.bh() * s.dv, [&](const T *rout, T *Z) {
+            LaStepOutArgs<T> a;
+            a.ld = s.width(), a.pow = pow, a.qkv = x.v, a.yw = syw.v + s.n_state(), a.z = rout, a.out = Z;
+            a.lam = T(0) - T(1);
+            return ::ddg::la_step_output<T>(s, a, this->st);
+        });
     }
     void output(const Tn<T> &o)
     {
@@ -593,6 +723,105 @@ struct EvalExec : ExecBase<T> {
         if (this->err == DDG_OK) ok(concat_rows<T>(av, bv, t.v, this->B, PROT, PROT, this->st));
         return t;
     }
+    // a product of wires: `word` writes this party's share from its key word, and it is opened
+    template <class F>
+    Tn<T> product(uint64_t n, F &&word)
+    {
+        const T *Z = reinterpret_cast<const T *>(key_at(words(n)));
+        T *sh = alloc(n);
+        if (this->err == DDG_OK) ok(word(Z, sh));
+        Tn<T> t;
+        t.n = n;
+        open_to(t, sh);
+        return t;
+    }
+    T one() const { return p == 0 ? T(1) : T(0); }
+    Tn<T> fc_q4(const Tn<T> &x, const Q4Layer<T> &w, int M)
+    {
+        const uint64_t n = uint64_t(M) * w.w.N;
+        const T *C = reinterpret_cast<const T *>(key_at(words(n)));
+        const T *sh = C;  // party 1's share is its key words
+        if (p == 0) {
+            const T *xv = val(x);
+            T *s0 = alloc(n);
+            if (this->err == DDG_OK) {
+                Q4Args<T> a;
+                a.w = w.w, a.M = M, a.x = xv, a.ldx = w.w.K, a.bias = w.b2s, a.Add = C, a.out = s0;
+                ok(::ddg::fc_q4<T>(a, this->st));
+            }
+            sh = s0;
+        }
+        Tn<T> t;
+        t.n = n;
+        open_to(t, sh);
+        return t;
+    }
+    Tn<T> floor_in(const Tn<T> &x) { return x; }
+    void floor_out(Tn<T> &) {}
+    Tn<T> la_decay(const LaShape &s, const T *pow, const Tn<T> &x)
+    {
+        Tn<T> t;
+        t.n = 2 * s.n_decayed();
+        const T *xv = val(x);
+        t.v = alloc(t.n);
+        if (this->err == DDG_OK) ok(::ddg::la_decay<T>(s, s.width(), pow, xv, t.v, this->st));
+        return t;
+    }
+    Tn<T> la_chunk(const LaShape &s, Tn<T> &x, Tn<T> &qk)
+    {
+        ensure_ms(x), ensure_ms(qk);
+        const T *xv = val(x), *kv = val(qk);
+        return product(s.n_ps(), [&](const T *Z, T *sh) {
+            LaChunkArgs<T> a;
+            a.ld = s.width(), a.qkv = xv, a.qkv_ms = x.ms0, a.kd = kv + s.n_decayed(), a.kd_ms = qk.ms0 + s.n_decayed();
+            a.z = Z, a.out = sh, a.p0 = one();
+            return ::ddg::la_chunk<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_carry(const LaShape &s, const T *pow, const Tn<T> &ps, const Tn<T> *s0)
+    {
+        Tn<T> t;
+        t.n = s.n_ps();
+        const T *pv = val(ps), *sv = s0 ? val(*s0) : nullptr;
+        t.v = alloc(t.n);
+        if (this->err == DDG_OK) ok(::ddg::la_carry<T>(s, pow, pv, sv, t.v, this->st));
+        return t;
+    }
+    Tn<T> la_output(const LaShape &s, Tn<T> &x, Tn<T> &qk, Tn<T> &ps, Tn<T> *s0)
+    {
+        ensure_ms(ps);
+        if (s0) ensure_ms(*s0);
+        const T *xv = val(x), *qv = val(qk), *pv = val(ps), *sv = s0 ? val(*s0) : nullptr;
+        return product(s.n_out(), [&](const T *Z, T *sh) {
+            LaOutArgs<T> a;
+            a.ld = s.width(), a.qkv = xv, a.qkv_ms = x.ms0, a.qd = qv, a.qd_ms = qk.ms0, a.ps = pv, a.ps_ms = ps.ms0;
+            a.s0 = sv, a.s0_ms = s0 ? s0->ms0 : nullptr, a.z = Z, a.out = sh, a.p0 = one();
+            return ::ddg::la_output<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_step(const LaShape &s, const T *pow, Tn<T> &x, Tn<T> &S)
+    {
+        ensure_ms(x), ensure_ms(S);
+        const T *xv = val(x), *sv = val(S);
+        return product(s.n_step(), [&](const T *Z, T *sh) {
+            LaStepArgs<T> a;
+            a.ld = s.width(), a.pow = pow, a.qkv = xv, a.qkv_ms = x.ms0, a.s = sv, a.s_ms = S.ms0, a.z = Z, a.out = sh;
+            a.p0 = a.lam = one();
+            return ::ddg::la_step<T>(s, a, this->st);
+        });
+    }
+    Tn<T> la_step_output(const LaShape &s, const T *pow, Tn<T> &x, Tn<T> &syw)
+    {
+        ensure_ms(syw);
+        const T *xv = val(x), *yv = val(syw);
+        return product(s.bh() * s.dv, [&](const T *Z, T *sh) {
+            LaStepOutArgs<T> a;
+            a.ld = s.width(), a.pow = pow, a.qkv = xv, a.qkv_ms = x.ms0;
+            a.yw = yv + s.n_state(), a.yw_ms = syw.ms0 + s.n_state(), a.z = Z, a.out = sh;
+            a.p0 = a.lam = one();
+            return ::ddg::la_step_output<T>(s, a, this->st);
+        });
+    }
     void output(const Tn<T> &o)
     {
         const T *r = reinterpret_cast<const T *>(key_at(words(o.n)));
@@ -689,6 +918,51 @@ Tn<T> fc_layer(E &x, Tn<T> &in, int l, int rows, int act)
     if (act == FC_ACT_RELU) return x.gate(graph_kinds().relu_ars, z);
     if (act == FC_ACT_TRUNC) return x.gate(GATE_ARS, z);
     return z;
+}
+
+// ---- the token model's layers (ddg_op_fc_q4_*, ddg_linattn_*)
+
+// floor(x / 2^s) for x in [-2^(bw-2), 2^(bw-2)) through the non-negative truncation gate
+template <typename T, class E>
+Tn<T> floor_gate(E &x, const Tn<T> &in)
+{
+    Tn<T> y = x.gate(graph_kinds().lrs, x.floor_in(in));
+    x.floor_out(y);
+    return y;
+}
+
+constexpr int FC_ACT_FLOOR = 3;
+
+template <typename T, class E>
+Tn<T> fc_q4_layer(E &x, Tn<T> &in, const Q4Layer<T> &w, int rows, int act)
+{
+    Tn<T> z = x.fc_q4(in, w, rows);
+    if (act == FC_ACT_RELU) return x.gate(graph_kinds().relu_ars, z);
+    if (act == FC_ACT_TRUNC) return x.gate(GATE_ARS, z);
+    if (act == FC_ACT_FLOOR) return floor_gate<T>(x, z);
+    return z;
+}
+
+// one prompt; s0 may be null; state: the state after its last token
+template <typename T, class E>
+Tn<T> linattn_layer(E &x, const LaShape &s, const T *pow, Tn<T> &qkv, Tn<T> *s0, Tn<T> &state)
+{
+    Tn<T> qk = floor_gate<T>(x, x.la_decay(s, pow, qkv));
+    Tn<T> own = floor_gate<T>(x, x.la_chunk(s, qkv, qk));
+    Tn<T> ps = floor_gate<T>(x, x.la_carry(s, pow, own, s0));
+    Tn<T> o = floor_gate<T>(x, x.la_output(s, qkv, qk, ps, s0));
+    state = slice(ps, ps.n - s.n_state(), s.n_state());
+    return o;
+}
+
+// one token per sequence
+template <typename T, class E>
+Tn<T> linattn_step_layer(E &x, const LaShape &s, const T *pow, Tn<T> &qkv, Tn<T> &S, Tn<T> &state)
+{
+    Tn<T> syw = floor_gate<T>(x, x.la_step(s, pow, qkv, S));
+    Tn<T> o = floor_gate<T>(x, x.la_step_output(s, pow, qkv, syw));
+    state = slice(syw, 0, s.n_state());
+    return o;
 }
 
 // GPUConcat (deepdtagen.h:45-100): reveal the public protein leaf (mask 0)

@@ -121,14 +121,14 @@ int run_eval(ddg_party *h, ddg_cursor *cur, int batch, F &&body)
     return DDG_OK;
 }
 
-int eval_ready(ddg_party *h, ddg_cursor *cur, int batch)
+int eval_ready(ddg_party *h, ddg_cursor *cur, int batch, bool weights = true)
 {
     DDG_CHECK(h && cur, DDG_ERR_ARG, "null party or cursor");
     DDG_CHECK(batch > 0, DDG_ERR_ARG, "batch must be positive (got %d)", batch);
     Party &P = h->P;
     DDG_CHECK(P.chan, DDG_ERR_STATE, "party %d has no channel", P.party);
     DDG_CHECK(P.keys, DDG_ERR_STATE, "party %d has no keys bound", P.party);
-    DDG_CHECK(P.w.table, DDG_ERR_STATE, "party %d has no weights", P.party);
+    DDG_CHECK(!weights || P.w.table, DDG_ERR_STATE, "party %d has no weights", P.party);
     DDG_CUDA(cudaSetDevice(P.device));
     DDG_TRY(keep_pool_memory(P.device));
     return aes_device_init();
@@ -178,6 +178,66 @@ int check_gate_kind(int kind, int bw, int s)
     return DDG_OK;
 }
 
+// the token model's layers: the ring and scale of the floors, then the layer's own sizes
+int check_floor(int bw, int s)
+{
+    DDG_CHECK(bw == 32 || bw == 64, DDG_ERR_ARG, "bw must be 32 or 64 (got %d)", bw);
+    DDG_CHECK(s >= 2 && s < bw - 2, DDG_ERR_ARG, "scale %d out of range for the floors at bw %d", s, bw);
+    return check_gate_kind(graph_kinds().lrs, bw, s);
+}
+
+int check_fc_q4(const ddg_q4_weights *w, int bw, int s, int rows, int act)
+{
+    DDG_TRY(check_q4(w));
+    DDG_CHECK(w->K > 0 && w->N > 0 && rows > 0, DDG_ERR_ARG, "bad FC sizes (%d rows, %d x %d)", rows, w->K, w->N);
+    DDG_CHECK(act_ok(act) || act == FC_ACT_FLOOR, DDG_ERR_ARG, "act %d out of range", act);
+    if (act == FC_ACT_FLOOR) return check_floor(bw, s);
+    return act == FC_ACT_RELU ? check_gate_kind(graph_kinds().relu_ars, bw, s) : DDG_OK;
+}
+
+int check_la_layer(const ddg_linattn_shape *p, int bw, int s, bool step, LaShape *out)
+{
+    DDG_TRY(check_linattn(p, out));
+    DDG_CHECK(out->B > 0 && out->T > 0, DDG_ERR_ARG, "batch and tokens must be positive (got %d, %d)", out->B, out->T);
+    DDG_CHECK(!step || out->T == 1, DDG_ERR_ARG, "a step takes one token per sequence (got %d)", out->T);
+    return check_floor(bw, s);
+}
+
+template <class W>
+int check_la_wires(const LaShape &s, const W *qkv, const W *s0)
+{
+    DDG_CHECK(qkv->n == uint64_t(s.n_qkv()), DDG_ERR_ARG, "the q|k|v wire holds %llu elements, not %lld",
+              (unsigned long long)qkv->n, (long long)s.n_qkv());
+    DDG_CHECK(!s0 || s0->n == uint64_t(s.n_state()), DDG_ERR_ARG, "the state wire holds %llu elements, not %lld",
+              (unsigned long long)s0->n, (long long)s.n_state());
+    return DDG_OK;
+}
+
+template <typename T>
+Q4Layer<T> q4_of(const ddg_q4_weights *w)
+{
+    Q4Layer<T> l;
+    l.w.K = w->K, l.w.N = w->N, l.w.group = w->group;
+    l.w.q = static_cast<const uint8_t *>(w->d_q), l.w.step = static_cast<const uint16_t *>(w->d_step);
+    l.b2s = static_cast<const T *>(w->d_bias2s);
+    return l;
+}
+
+template <class F32, class F64>
+uint64_t key_bytes_of(int bw, int s, F32 &&f32, F64 &&f64)
+{
+    if (bw == 32) {
+        SizeExec<uint32_t> e;
+        e.bw = bw, e.s = s;
+        f32(e);
+        return align256(e.off);
+    }
+    SizeExec<uint64_t> e;
+    e.bw = bw, e.s = s;
+    f64(e);
+    return align256(e.off);
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ evaluators
@@ -193,7 +253,7 @@ extern "C" {
 
 int ddg_op_input_eval(ddg_party *h, ddg_cursor *cur, uint64_t n, const void *d_share, ddg_wire *out)
 {
-    DDG_TRY(eval_ready(h, cur, 1));
+    DDG_TRY(eval_ready(h, cur, 1, false));
     DDG_TRY(check_wires({d_share, out, out ? out->d_value : nullptr}));
 #define BODY(T)                                     \
     e.in[IN_X] = static_cast<const T *>(d_share);   \
@@ -533,5 +593,144 @@ int ddg_op_output_keygen(ddg_dealer *d, ddg_cursor *cur, ddg_mask_wire *o)
     return DDG_DISPATCH_KEYGEN(d, cur, 1, BODY);
 #undef BODY
 }
+
+// ------------------------------------------------------------------ token model
+
+uint64_t ddg_op_fc_q4_key_bytes(int bw, int scale, int K, int N, int rows, int act)
+{
+    const void *some = reinterpret_cast<const void *>(uintptr_t(256));  // sizes only: nothing is read
+    const ddg_q4_weights w = {K, N, 32, some, some, nullptr};
+    if ((bw != 32 && bw != 64) || scale < 1 || scale >= bw - 1) return 0;
+    if (check_fc_q4(&w, bw, scale, rows, act) != DDG_OK) return 0;
+#define BODY(T)                                                    \
+    [&](SizeExec<T> &e) {                                          \
+        Tn<T> x = e.mk(uint64_t(rows) * K);                        \
+        fc_q4_layer<T>(e, x, q4_of<T>(&w), rows, act);             \
+    }
+    return key_bytes_of(bw, scale, BODY(uint32_t), BODY(uint64_t));
+#undef BODY
+}
+
+int ddg_op_fc_q4_eval(ddg_party *h, ddg_cursor *cur, const ddg_q4_weights *w, int rows, int act, ddg_wire *x,
+                      ddg_wire *out)
+{
+    DDG_TRY(eval_ready(h, cur, 1, false));
+    DDG_TRY(check_wires({x, out, x ? x->d_value : nullptr, out ? out->d_value : nullptr}));
+    DDG_TRY(check_fc_q4(w, h->P.bw, h->P.s, rows, act));
+    DDG_CHECK(x->n == uint64_t(rows) * w->K, DDG_ERR_ARG, "FC input is not %d x %d", rows, w->K);
+#define BODY(T)                                                    \
+    Tn<T> X = tn_of<T>(x);                                         \
+    Tn<T> y = fc_q4_layer<T>(e, X, q4_of<T>(w), rows, act);        \
+    put<T>(e, out, y);
+    return DDG_DISPATCH_EVAL(h, cur, 1, BODY);
+#undef BODY
+}
+
+int ddg_op_fc_q4_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_q4_weights *w, int rows, int act,
+                        ddg_mask_wire *x, ddg_mask_wire *out)
+{
+    DDG_TRY(keygen_ready(d, cur, 1));
+    DDG_TRY(check_wires({x, out, x ? x->d_mask : nullptr, out ? out->d_mask : nullptr}));
+    DDG_TRY(check_fc_q4(w, d->bw, d->s, rows, act));
+    DDG_CHECK(x->n == uint64_t(rows) * w->K, DDG_ERR_ARG, "FC input is not %d x %d", rows, w->K);
+#define BODY(T)                                                    \
+    Tn<T> X = tn_of<T>(x);                                         \
+    Tn<T> y = fc_q4_layer<T>(e, X, q4_of<T>(w), rows, act);        \
+    put<T>(e, out, y);
+    return DDG_DISPATCH_KEYGEN(d, cur, 1, BODY);
+#undef BODY
+}
+
+uint64_t ddg_linattn_key_bytes(int bw, int scale, const ddg_linattn_shape *shape, int with_s0)
+{
+    LaShape s;
+    if (check_la_layer(shape, bw, scale, false, &s) != DDG_OK) return 0;
+#define BODY(T)                                                                        \
+    [&](SizeExec<T> &e) {                                                              \
+        Tn<T> x = e.mk(s.n_qkv()), s0 = e.mk(s.n_state()), state;                      \
+        linattn_layer<T>(e, s, nullptr, x, with_s0 ? &s0 : nullptr, state);            \
+    }
+    return key_bytes_of(bw, scale, BODY(uint32_t), BODY(uint64_t));
+#undef BODY
+}
+
+#define LA_BODY(T)                                                                     \
+    Tn<T> X = tn_of<T>(qkv), S, state;                                                 \
+    if (s0) S = tn_of<T>(s0);                                                          \
+    Tn<T> y = linattn_layer<T>(e, s, static_cast<const T *>(d_pow), X, s0 ? &S : nullptr, state); \
+    back<T>(qkv, X);                                                                   \
+    if (s0) back<T>(s0, S);                                                            \
+    put<T>(e, out, y);                                                                 \
+    put<T>(e, state_out, state);
+
+int ddg_linattn_eval(ddg_party *h, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                     ddg_wire *qkv, ddg_wire *s0, ddg_wire *out, ddg_wire *state_out)
+{
+    LaShape s;
+    DDG_TRY(eval_ready(h, cur, 1, false));
+    DDG_TRY(check_la_layer(shape, h->P.bw, h->P.s, false, &s));
+    DDG_TRY(check_wires({d_pow, qkv, out, state_out, qkv ? qkv->d_value : nullptr, out ? out->d_value : nullptr,
+                         state_out ? state_out->d_value : nullptr, s0 ? s0->d_value : d_pow}));
+    DDG_TRY(check_la_wires(s, qkv, s0));
+    return DDG_DISPATCH_EVAL(h, cur, s.B, LA_BODY);
+}
+
+int ddg_linattn_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                       ddg_mask_wire *qkv, ddg_mask_wire *s0, ddg_mask_wire *out, ddg_mask_wire *state_out)
+{
+    LaShape s;
+    DDG_TRY(keygen_ready(d, cur, 1));
+    DDG_TRY(check_la_layer(shape, d->bw, d->s, false, &s));
+    DDG_TRY(check_wires({d_pow, qkv, out, state_out, qkv ? qkv->d_mask : nullptr, out ? out->d_mask : nullptr,
+                         state_out ? state_out->d_mask : nullptr, s0 ? s0->d_mask : d_pow}));
+    DDG_TRY(check_la_wires(s, qkv, s0));
+    return DDG_DISPATCH_KEYGEN(d, cur, s.B, LA_BODY);
+}
+#undef LA_BODY
+
+uint64_t ddg_linattn_step_key_bytes(int bw, int scale, const ddg_linattn_shape *shape)
+{
+    LaShape s;
+    if (check_la_layer(shape, bw, scale, true, &s) != DDG_OK) return 0;
+#define BODY(T)                                                                        \
+    [&](SizeExec<T> &e) {                                                              \
+        Tn<T> x = e.mk(s.n_qkv()), S = e.mk(s.n_state()), state;                       \
+        linattn_step_layer<T>(e, s, nullptr, x, S, state);                             \
+    }
+    return key_bytes_of(bw, scale, BODY(uint32_t), BODY(uint64_t));
+#undef BODY
+}
+
+#define LA_BODY(T)                                                                     \
+    Tn<T> X = tn_of<T>(qkv), S = tn_of<T>(s_in), state;                                \
+    Tn<T> y = linattn_step_layer<T>(e, s, static_cast<const T *>(d_pow), X, S, state); \
+    back<T>(qkv, X), back<T>(s_in, S);                                                 \
+    put<T>(e, out, y);                                                                 \
+    put<T>(e, state_out, state);
+
+int ddg_linattn_step_eval(ddg_party *h, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                          ddg_wire *qkv, ddg_wire *s_in, ddg_wire *out, ddg_wire *state_out)
+{
+    LaShape s;
+    DDG_TRY(eval_ready(h, cur, 1, false));
+    DDG_TRY(check_la_layer(shape, h->P.bw, h->P.s, true, &s));
+    DDG_TRY(check_wires({d_pow, qkv, s_in, out, state_out, qkv ? qkv->d_value : nullptr, s_in ? s_in->d_value : nullptr,
+                         out ? out->d_value : nullptr, state_out ? state_out->d_value : nullptr}));
+    DDG_TRY(check_la_wires(s, qkv, s_in));
+    return DDG_DISPATCH_EVAL(h, cur, s.B, LA_BODY);
+}
+
+int ddg_linattn_step_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                            ddg_mask_wire *qkv, ddg_mask_wire *s_in, ddg_mask_wire *out, ddg_mask_wire *state_out)
+{
+    LaShape s;
+    DDG_TRY(keygen_ready(d, cur, 1));
+    DDG_TRY(check_la_layer(shape, d->bw, d->s, true, &s));
+    DDG_TRY(check_wires({d_pow, qkv, s_in, out, state_out, qkv ? qkv->d_mask : nullptr, s_in ? s_in->d_mask : nullptr,
+                         out ? out->d_mask : nullptr, state_out ? state_out->d_mask : nullptr}));
+    DDG_TRY(check_la_wires(s, qkv, s_in));
+    return DDG_DISPATCH_KEYGEN(d, cur, s.B, LA_BODY);
+}
+#undef LA_BODY
 
 }  // extern "C"

@@ -65,6 +65,9 @@ template <typename T>
 int ew_add(T *out, const T *a, const T *b, uint64_t n, cudaStream_t st);
 template <typename T>
 int ew_sub(T *out, const T *a, const T *b, uint64_t n, cudaStream_t st);
+// out[i] = a[i] + c (out may be a)
+template <typename T>
+int ew_offset(T *out, const T *a, T c, uint64_t n, cudaStream_t st);
 
 // party share of x*y: p0*xh*yh - xh*[r_y] - [r_x]*yh + Z (xh2, yh2: second
 // addends of the opened inputs, or null)

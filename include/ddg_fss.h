@@ -485,6 +485,124 @@ int ddg_op_concat_protein_keygen(ddg_dealer *dealer, ddg_cursor *cur, int batch,
 int ddg_op_output_keygen(ddg_dealer *dealer, ddg_cursor *cur, ddg_mask_wire *o);
 
 /* ------------------------------------------------------------------------
+ * Operators of a secure token model: fully connected layers with 4-bit
+ * public weights, and linear attention with a decay per head.  The share
+ * calls are one party's local computation between two openings, like
+ * ddg_fc_share and ddg_matmul_share; the wire calls (ddg_op_fc_q4_*,
+ * ddg_linattn_*, ddg_linattn_step_*) run them with their openings and
+ * truncation gates over the party's channel, like ddg_op_fc_*.  No counterpart
+ * in the reference, whose model ends at the affinity head.
+ * ---------------------------------------------------------------------- */
+
+/* Public 4-bit weights of a (K x N) layer:
+ *   W[k][n] = step[k / group][n] * (code(n, k) - 8)     at the fixed-point scale
+ * d_q: output n's codes in one row of ddg_q4_row_bytes(K) bytes, code k in the
+ * low half (k even) or the high half (k odd) of byte k/2; 16-byte aligned.
+ * d_step: ceil(K / group) x N uint16 steps of 12 bits (higher bits are
+ * ignored), so that every weight is below 2^15 in magnitude.  group is a
+ * multiple of 32.  d_bias2s: N ring elements (bias << scale), or NULL. */
+typedef struct ddg_q4_weights {
+    int K, N, group;
+    const void *d_q;
+    const void *d_step;
+    const void *d_bias2s;
+} ddg_q4_weights;
+uint64_t ddg_q4_row_bytes(int K); /* 16 * ceil(K / 32); 0 for K < 1 */
+/* codes and steps of an int64 device matrix d_w (K x N, row-major, at the
+ * fixed-point scale, as in weights.bin): per group and output the smallest
+ * step that brings every weight into -7..7, codes rounded to nearest, halves
+ * away from zero.  A group whose largest weight exceeds 7 * 4095 gets step
+ * 4095 and saturates at -8 / 7. */
+int ddg_q4_quantize(int K, int N, int group, const int64_t *d_w, void *d_q, void *d_step, void *stream);
+/* as ddg_fc_share with 4-bit weights, rows of x_hat ldx elements apart:
+ *   party 0: out = x_hat . W + bias2s + C0;  party 1: out = C1
+ * d_c and d_out (M x N) contiguous; d_out may be d_c. */
+int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const void *d_xhat, int64_t ldx,
+                    const void *d_c, void *d_out, void *stream);
+
+/* Linear attention  S_t = lambda_h S_{t-1} + k_t v_t^T,  o_t = q_t S_t  (S is
+ * dk x dv per head), for prompts in chunks of `chunk` tokens and for one token.
+ * batch >= 0, heads >= 1, tokens >= 0, dk, dv and chunk in 1..128; pow_n >=
+ * tokens and >= 1.  Arrays, row-major, T = tokens, bh = batch * heads + head:
+ *   qkv     (batch, T) rows, ld elements apart, each [q: heads x dk |
+ *           k: heads x dk | v: heads x dv], ld >= heads * (2 dk + dv)
+ *   pow     (heads, pow_n + 1): lambda_h^n at the scale (ddg_decay_table)
+ *   qkd     [Qd (batch*heads, T, dk) | Kd (batch*heads, T, dk)]
+ *   ps      [P (batch*heads, tri) | S (chunks, batch*heads, dk, dv)], where
+ *           tri lists, chunk by chunk, the rows i = 0, 1, .. of a causal
+ *           triangle, i + 1 entries each
+ *   state   (batch*heads, dk, dv);  out (batch, T, heads, dv)
+ * With fl(x) = floor(x / 2^scale), len(c) and end(c) the length and end of
+ * chunk c, i and j tokens of one chunk, a prompt is
+ *   [Qd | Kd] = fl(ddg_linattn_decay)          pow[i+1] q_i | pow[len-1-i] k_i
+ *   [P | S']  = fl(ddg_linattn_chunk_share)    q_i . k_j (j <= i) | Kd^T . V
+ *   [P | S]   = fl(ddg_linattn_carry)          pow[i-j] P_ij |
+ *               S_c = sum_{c' <= c} pow[end(c)-end(c')] S'_{c'} + pow[end(c)] S0
+ *   out       = fl(ddg_linattn_output_share)   P . V + Qd . S_{c-1}  (S_{-1} = S0)
+ * whose state after the prompt is S of its last chunk, and one token is
+ *   [S | y | w] = fl(ddg_linattn_step_share)   lambda S + k v^T | q . S | q . k
+ *   out         = fl(ddg_linattn_step_output_share)   lambda y + w v
+ * (y: (batch*heads, dv), w: (batch*heads)).  Every stage is exact modulo 2^bw. */
+typedef struct ddg_linattn_shape {
+    int batch, heads, tokens, dk, dv, chunk, pow_n;
+} ddg_linattn_shape;
+/* host: h_pow (heads x (n + 1) ring elements) = round(lambda^i * 2^scale), h_lambda in [0, 1] */
+int ddg_decay_table(int bw, int scale, int heads, int n, const double *h_lambda, void *h_pow);
+/* array sizes in ring elements: out6 = {qkv at the least ld, qkd, ps, state, step output, out} */
+int ddg_linattn_sizes(const ddg_linattn_shape *shape, int64_t *out6);
+/* the two public maps: on a masked value the masked result, on the dealer's
+ * mask the result's mask (no key).  d_s0 may be NULL (a zero state). */
+int ddg_linattn_decay(int bw, const ddg_linattn_shape *shape, int64_t ld, const void *d_pow, const void *d_qkv,
+                      void *d_out, void *stream);
+int ddg_linattn_carry(int bw, const ddg_linattn_shape *shape, const void *d_pow, const void *d_ps, const void *d_s0,
+                      void *d_out, void *stream);
+/* the products: masked values (_hat), the party's mask shares (_ms) and its
+ * share d_z of the dealer's word (mask product - lambda * mask of S or y, plus
+ * the output mask); d_out, the party's share of the masked result, overlaps
+ * no input but d_z. */
+int ddg_linattn_chunk_share(int bw, int party, const ddg_linattn_shape *shape, int64_t ld, const void *d_qkv_hat,
+                            const void *d_qkv_ms, const void *d_kd_hat, const void *d_kd_ms, const void *d_z,
+                            void *d_out, void *stream);
+int ddg_linattn_output_share(int bw, int party, const ddg_linattn_shape *shape, int64_t ld, const void *d_qkv_hat,
+                             const void *d_qkv_ms, const void *d_qd_hat, const void *d_qd_ms, const void *d_ps_hat,
+                             const void *d_ps_ms, const void *d_s0_hat, const void *d_s0_ms, const void *d_z,
+                             void *d_out, void *stream);
+int ddg_linattn_step_share(int bw, int party, const ddg_linattn_shape *shape, int64_t ld, const void *d_pow,
+                           const void *d_qkv_hat, const void *d_qkv_ms, const void *d_s_hat, const void *d_s_ms,
+                           const void *d_z, void *d_out, void *stream);
+int ddg_linattn_step_output_share(int bw, int party, const ddg_linattn_shape *shape, int64_t ld, const void *d_pow,
+                                  const void *d_qkv_hat, const void *d_qkv_ms, const void *d_yw_hat,
+                                  const void *d_yw_ms, const void *d_z, void *d_out, void *stream);
+
+/* The same on wires, with the openings and the gates (both parties make the
+ * same calls; no affinity weights are needed).  The floors after the products
+ * are exact for values in [-2^(bw-2), 2^(bw-2)): the dealer shifts the masks
+ * of the non-negative truncation gate by 2^(bw-2).  2 <= scale < bw - 2.
+ * act: DDG_ACT_NONE, DDG_ACT_RELU, DDG_ACT_TRUNC as in ddg_op_fc_*, or
+ * DDG_ACT_FLOOR, the floor just described (a tenth of DDG_ACT_TRUNC's key
+ * bytes).  d_pow and the members of w are device arrays, the same on the
+ * dealer and both parties.  Prompts and steps take the state as a wire and
+ * give it back as one; a prompt's s0 may be NULL.  The key-byte functions count
+ * from a 256-byte boundary and include the inputs' mask shares, which a call
+ * reads only for a wire that has none yet; 0 for bad arguments. */
+#define DDG_ACT_FLOOR 3
+uint64_t ddg_op_fc_q4_key_bytes(int bw, int scale, int K, int N, int rows, int act);
+int ddg_op_fc_q4_keygen(ddg_dealer *dealer, ddg_cursor *cur, const ddg_q4_weights *w, int rows, int act,
+                        ddg_mask_wire *x, ddg_mask_wire *out);
+int ddg_op_fc_q4_eval(ddg_party *party, ddg_cursor *cur, const ddg_q4_weights *w, int rows, int act, ddg_wire *x,
+                      ddg_wire *out);
+uint64_t ddg_linattn_key_bytes(int bw, int scale, const ddg_linattn_shape *shape, int with_s0);
+int ddg_linattn_keygen(ddg_dealer *dealer, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                       ddg_mask_wire *qkv, ddg_mask_wire *s0, ddg_mask_wire *out, ddg_mask_wire *state);
+int ddg_linattn_eval(ddg_party *party, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                     ddg_wire *qkv, ddg_wire *s0, ddg_wire *out, ddg_wire *state);
+uint64_t ddg_linattn_step_key_bytes(int bw, int scale, const ddg_linattn_shape *shape);
+int ddg_linattn_step_keygen(ddg_dealer *dealer, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                            ddg_mask_wire *qkv, ddg_mask_wire *s, ddg_mask_wire *out, ddg_mask_wire *state);
+int ddg_linattn_step_eval(ddg_party *party, ddg_cursor *cur, const ddg_linattn_shape *shape, const void *d_pow,
+                          ddg_wire *qkv, ddg_wire *s, ddg_wire *out, ddg_wire *state);
+
+/* ------------------------------------------------------------------------
  * Key chunks and streaming (replaces the chunked key file and the streaming
  * evaluation of deepdtagen_inference.cu:344-416 and :608-826: 4 KiB-padded
  * chunks, 2 pinned + 2 device slots, a copy stream and events).
