@@ -29,6 +29,9 @@ int la_grid(int64_t n)
     return int(b < 148 * 64 ? (b ? b : 1) : 148 * 64);
 }
 
+// blocks of LA_THREADS threads with V of n elements each
+inline int64_t la_blocks(int64_t n, int V) { return (n + int64_t(LA_THREADS) * V - 1) / (int64_t(LA_THREADS) * V); }
+
 #define LA_EACH(e, n) \
     for (int64_t e = int64_t(blockIdx.x) * LA_THREADS + threadIdx.x; e < (n); e += int64_t(gridDim.x) * LA_THREADS)
 
@@ -44,28 +47,123 @@ __device__ __forceinline__ void tri_find(const LaShape &s, int64_t e, int &c, in
     j = r - i * (i + 1) / 2;
 }
 
+// V elements moved together: 16 bytes, or single elements where rows do not allow it
+template <typename T, int V>
+struct alignas(V * sizeof(T)) Pack {
+    T e[V];
+};
 template <typename T>
-__device__ __forceinline__ const T *qkv_row(const LaShape &s, int64_t ld, const T *x, int64_t b, int64_t t)
-{
-    return x + (b * s.T + t) * ld;
-}
+constexpr int VEC = 16 / int(sizeof(T));
 
-template <typename T>
+inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ------------------------------------------------------------------ public maps (memory-bound)
+
+// One token per block step: its q and k are one contiguous run, written as dk-long runs per head.
+template <typename T, int V>
 __global__ void __launch_bounds__(LA_THREADS)
     k_la_decay(const LaShape s, int64_t ld, const T *pow, const T *x, T *out)
 {
-    const int64_t nd = s.n_decayed();
-    LA_EACH(e, 2 * nd)
-    {
-        const bool key = e >= nd;
-        const int64_t r = key ? e - nd : e;
-        const int d = int(r % s.dk);
-        const int64_t bt = r / s.dk;
-        const int t = int(bt % s.T);
-        const int64_t bh = bt / s.T, b = bh / s.H;
-        const int h = int(bh % s.H), c = t / s.C, i = t - c * s.C;
-        const T *row = qkv_row(s, ld, x, b, t) + (key ? int64_t(s.H) * s.dk : 0) + int64_t(h) * s.dk;
-        out[e] = pow[int64_t(h) * (s.pn + 1) + (key ? s.len(c) - 1 - i : i + 1)] * row[d];
+    const int dkv = s.dk / V, half = s.H * dkv;
+    const int64_t tokens = int64_t(s.B) * s.T, nd = s.n_decayed();
+    for (int64_t bt = blockIdx.x; bt < tokens; bt += gridDim.x) {
+        const int64_t b = bt / s.T;
+        const int t = int(bt - b * s.T), c = t / s.C, i = t - c * s.C, back = s.len(c) - 1 - i;
+        const Pack<T, V> *row = reinterpret_cast<const Pack<T, V> *>(x + bt * ld);
+        for (int e = threadIdx.x; e < 2 * half; e += LA_THREADS) {
+            const bool key = e >= half;
+            const int r = key ? e - half : e, h = r / dkv, d = r - h * dkv;
+            const T p = __ldg(pow + int64_t(h) * (s.pn + 1) + (key ? back : i + 1));
+            Pack<T, V> v = row[e];
+#pragma unroll
+            for (int j = 0; j < V; j++) v.e[j] *= p;
+            reinterpret_cast<Pack<T, V> *>(out + (key ? nd : 0) + ((b * s.H + h) * s.T + t) * s.dk)[d] = v;
+        }
+    }
+}
+
+// Scores: V consecutive packed entries per thread, the triangle walked from the
+// first one's position.  States: V columns of up to LC_OT output chunks per
+// thread, every earlier chunk read once per LC_OT outputs; the sums cannot
+// be chained from chunk to chunk, because each S_c is floored from exact terms.
+constexpr int LC_OT = 16;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(LA_THREADS)
+    k_la_carry(const LaShape s, const T *pow, const T *ps, const T *s0, T *out, int score_blocks)
+{
+    const int64_t ns = s.n_scores(), tri = s.tri();
+    if (int(blockIdx.x) < score_blocks) {
+        for (int64_t e0 = (int64_t(blockIdx.x) * LA_THREADS + threadIdx.x) * V; e0 < ns;
+             e0 += int64_t(score_blocks) * LA_THREADS * V) {
+            int64_t bh = e0 / tri;
+            int c, i, j;
+            tri_find(s, e0 - bh * tri, c, i, j);
+            const int n = ns - e0 < V ? int(ns - e0) : V;
+            Pack<T, V> v;
+            if (n == V)
+                v = *reinterpret_cast<const Pack<T, V> *>(ps + e0);
+            else
+                for (int k = 0; k < n; k++) v.e[k] = ps[e0 + k];
+            const T *pw = pow + bh % s.H * (s.pn + 1);
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                if (k >= n) break;
+                v.e[k] *= __ldg(pw + i - j);
+                if (++j > i) {  // next row, chunk or head
+                    j = 0;
+                    if (++i >= s.len(c)) {
+                        i = 0;
+                        if (++c >= s.chunks()) c = 0, bh++, pw = pow + bh % s.H * (s.pn + 1);
+                    }
+                }
+            }
+            if (n == V)
+                *reinterpret_cast<Pack<T, V> *>(out + e0) = v;
+            else
+                for (int k = 0; k < n; k++) out[e0 + k] = v.e[k];
+        }
+        return;
+    }
+    const int64_t state = s.n_state(), per = int64_t(s.dk) * s.dv;
+    const int nc = s.chunks();
+    const int64_t r = (int64_t(blockIdx.x - score_blocks) * LA_THREADS + threadIdx.x) * V;
+    if (r >= state) return;
+    const T *const pw = pow + r / per % s.H * (s.pn + 1);
+    const T *const in = ps + ns + r;
+    Pack<T, V> first;
+#pragma unroll
+    for (int k = 0; k < V; k++) first.e[k] = 0;
+    if (s0) first = *reinterpret_cast<const Pack<T, V> *>(s0 + r);
+    for (int c0 = 0; c0 < nc; c0 += LC_OT) {
+        T acc[LC_OT][V];
+#pragma unroll
+        for (int o = 0; o < LC_OT; o++) {
+            const T p = c0 + o < nc ? __ldg(pw + s.end(c0 + o)) : T(0);
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[o][k] = p * first.e[k];
+        }
+        const int jn = c0 + LC_OT < nc ? c0 + LC_OT : nc;
+        for (int j = 0; j < jn; j++) {
+            const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(in + j * state);
+            const int at = s.end(j);
+#pragma unroll
+            for (int o = 0; o < LC_OT; o++) {
+                if (c0 + o >= j && c0 + o < nc) {
+                    const T p = __ldg(pw + s.end(c0 + o) - at);
+#pragma unroll
+                    for (int k = 0; k < V; k++) acc[o][k] += p * v.e[k];
+                }
+            }
+        }
+#pragma unroll
+        for (int o = 0; o < LC_OT; o++) {
+            if (c0 + o >= nc) break;
+            Pack<T, V> v;
+#pragma unroll
+            for (int k = 0; k < V; k++) v.e[k] = acc[o][k];
+            *reinterpret_cast<Pack<T, V> *>(out + ns + (c0 + o) * state + r) = v;
+        }
     }
 }
 
@@ -359,29 +457,6 @@ __global__ void __launch_bounds__(LA_THREADS, 2)
 }
 
 template <typename T>
-__global__ void __launch_bounds__(LA_THREADS)
-    k_la_carry(const LaShape s, const T *pow, const T *ps, const T *s0, T *out)
-{
-    const int64_t ns = s.n_scores(), tri = s.tri(), state = s.n_state(), per = int64_t(s.dk) * s.dv;
-    LA_EACH(e, s.n_ps())
-    {
-        if (e < ns) {
-            const int64_t bh = e / tri;
-            int c, i, j;
-            tri_find(s, e - bh * tri, c, i, j);
-            out[e] = pow[(bh % s.H) * (s.pn + 1) + i - j] * ps[e];
-        } else {
-            const int64_t r = (e - ns) % state;
-            const int c = int((e - ns) / state), end = s.end(c);
-            const T *pw = pow + (r / per % s.H) * (s.pn + 1);
-            T acc = s0 ? pw[end] * s0[r] : T(0);
-            for (int j = 0; j <= c; j++) acc += pw[end - s.end(j)] * ps[ns + j * state + r];
-            out[e] = acc;
-        }
-    }
-}
-
-template <typename T>
 __global__ void __launch_bounds__(LA_THREADS, 2)
     k_la_output(const LaShape s, const __grid_constant__ LaOutArgs<T> a, int tiles, uint32_t *err)
 {
@@ -420,33 +495,81 @@ __global__ void __launch_bounds__(LA_THREADS, 2)
         len, [&](int i) { return o + int64_t(i) * s.H * s.dv; }, [&](int) { return s.dv - y0; }, a.z, a.out, err);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(LA_THREADS) k_la_step(const LaShape s, const __grid_constant__ LaStepArgs<T> a)
+// ------------------------------------------------------------------ one token
+//
+// A block takes CX x V columns of one head's state, its 256 / CX thread rows
+// stride over dk: S, its mask share and the dealer's word are read once and
+// the new state written once (4 words moved and 5 multiply-adds per entry, so
+// bound by memory); q . S comes out of the same pass, summed over the thread
+// rows in shared memory.
+template <typename T, int V>
+__global__ void __launch_bounds__(LA_THREADS)
+    k_la_step(const LaShape s, const __grid_constant__ LaStepArgs<T> a, int cx, int slabs)
 {
+    __shared__ T qs[128], ks[128], rq[128], rk[128];
+    __shared__ Pack<T, V> red[LA_THREADS];
+    using PV = Pack<T, V>;
+    const int64_t bh = blockIdx.x / slabs, b = bh / s.H;
+    const int slab = int(blockIdx.x - bh * slabs), h = int(bh - b * s.H), tid = threadIdx.x;
+    const int ry = LA_THREADS / cx, x = tid % cx, y0 = tid / cx, col = (slab * cx + x) * V;
     const int64_t state = s.n_state(), ny = s.bh() * s.dv, per = int64_t(s.dk) * s.dv;
-    LA_EACH(e, s.n_step())
-    {
-        const bool u = e < state, w = e >= state + ny;
-        const int64_t r = u ? e : w ? e - state - ny : e - state;
-        const int64_t bh = u ? r / per : w ? r : r / s.dv, b = bh / s.H, h = bh % s.H;
-        const int64_t oq = b * a.ld + h * s.dk, ok = oq + int64_t(s.H) * s.dk;
-        T acc = 0;
-        if (u) {
-            const int64_t x = ok + (r - bh * per) / s.dv;
-            const int64_t y = b * a.ld + 2 * int64_t(s.H) * s.dk + h * s.dv + r % s.dv;
-            T right = a.p0 * a.qkv[y];
-            if (a.qkv_ms) right -= a.qkv_ms[y], acc -= a.qkv_ms[x] * a.qkv[y];
-            acc += a.qkv[x] * right + a.lam * a.pow[h * (s.pn + 1) + 1] * a.s[r];
-        } else {
-            for (int x = 0; x < s.dk; x++) {
-                const int64_t os = bh * per + int64_t(x) * s.dv + r % s.dv;
-                const T b1 = w ? a.qkv[ok + x] : a.s[os];
-                T right = a.p0 * b1;
-                if (a.qkv_ms) right -= w ? a.qkv_ms[ok + x] : a.s_ms[os], acc -= a.qkv_ms[oq + x] * b1;
-                acc += a.qkv[oq + x] * right;
+    const int64_t oq = b * a.ld + int64_t(h) * s.dk, ok = oq + int64_t(s.H) * s.dk;
+    const int64_t ov = b * a.ld + 2 * int64_t(s.H) * s.dk + int64_t(h) * s.dv + col;
+    const bool on = col < s.dv;
+    T v[V], vr[V], acc[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+        v[k] = on ? __ldg(a.qkv + ov + k) : T(0);
+        vr[k] = a.p0 * v[k] - (on && a.qkv_ms ? __ldg(a.qkv_ms + ov + k) : T(0));
+        acc[k] = 0;
+    }
+    for (int i = tid; i < s.dk; i += LA_THREADS) {
+        qs[i] = __ldg(a.qkv + oq + i), ks[i] = __ldg(a.qkv + ok + i);
+        rq[i] = a.qkv_ms ? __ldg(a.qkv_ms + oq + i) : T(0), rk[i] = a.qkv_ms ? __ldg(a.qkv_ms + ok + i) : T(0);
+    }
+    const T lam = a.lam * __ldg(a.pow + int64_t(h) * (s.pn + 1) + 1);
+    __syncthreads();
+    if (on) {
+        const int64_t at = bh * per + col;
+#pragma unroll 4
+        for (int i = y0; i < s.dk; i += ry) {
+            const int64_t o = at + int64_t(i) * s.dv;
+            const PV S = *reinterpret_cast<const PV *>(a.s + o), z = *reinterpret_cast<const PV *>(a.z + o);
+            PV m, u;
+            if (a.qkv_ms)
+                m = *reinterpret_cast<const PV *>(a.s_ms + o);
+            else
+#pragma unroll
+                for (int k = 0; k < V; k++) m.e[k] = 0;
+            const T q = qs[i], key = ks[i], mq = rq[i], mk = rk[i];
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                u.e[k] = z.e[k] + lam * S.e[k] + key * vr[k] - mk * v[k];
+                acc[k] += q * (a.p0 * S.e[k] - m.e[k]) - mq * S.e[k];
             }
+            *reinterpret_cast<PV *>(a.out + o) = u;
         }
-        a.out[e] = acc + a.z[e];
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++) red[tid].e[k] = acc[k];
+    for (int half = ry / 2; half; half >>= 1) {
+        __syncthreads();
+        if (y0 < half)
+#pragma unroll
+            for (int k = 0; k < V; k++) red[tid].e[k] += red[tid + half * cx].e[k];
+    }
+    if (y0 == 0 && on)
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int64_t o = state + bh * s.dv + col + k;
+            a.out[o] = red[tid].e[k] + a.z[o];
+        }
+    if (slab == 0 && tid < 32) {
+        T w = 0;
+        for (int i = tid; i < s.dk; i += 32) w += qs[i] * (a.p0 * ks[i] - rk[i]) - rq[i] * ks[i];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        if (tid == 0) a.out[state + ny + bh] = w + a.z[state + ny + bh];
     }
 }
 
@@ -478,7 +601,13 @@ template <typename T>
 int la_decay(const LaShape &s, int64_t ld, const T *pow, const T *x, T *out, cudaStream_t st)
 {
     if (!s.n_decayed()) return DDG_OK;
-    k_la_decay<T><<<la_grid(2 * s.n_decayed()), LA_THREADS, 0, st>>>(s, ld, pow, x, out);
+    constexpr int V = VEC<T>;
+    const int64_t tokens = int64_t(s.B) * s.T;
+    const int grid = int(tokens < 148 * 16 ? tokens : 148 * 16);
+    if (s.dk % V == 0 && ld % V == 0 && al16(x) && al16(out))
+        k_la_decay<T, V><<<grid, LA_THREADS, 0, st>>>(s, ld, pow, x, out);
+    else
+        k_la_decay<T, 1><<<grid, LA_THREADS, 0, st>>>(s, ld, pow, x, out);
     return launched();
 }
 
@@ -510,12 +639,26 @@ int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
     return launched();
 }
 
+template <typename T, int V>
+static int launch_carry(const LaShape &s, const T *pow, const T *ps, const T *s0, T *out, cudaStream_t st)
+{
+    const int64_t sb = la_blocks(s.n_scores(), V), nb = la_blocks(s.n_state(), V);
+    const int score_blocks = int(sb < 148 * 16 ? sb : 148 * 16);
+    DDG_CHECK(nb + score_blocks <= 0x7fffffff, DDG_ERR_ARG, "linear attention: %lld state entries are too many",
+              (long long)s.n_state());
+    k_la_carry<T, V><<<unsigned(score_blocks + nb), LA_THREADS, 0, st>>>(s, pow, ps, s0, out, score_blocks);
+    return launched();
+}
+
 template <typename T>
 int la_carry(const LaShape &s, const T *pow, const T *ps, const T *s0, T *out, cudaStream_t st)
 {
     if (!s.n_ps()) return DDG_OK;
-    k_la_carry<T><<<la_grid(s.n_ps()), LA_THREADS, 0, st>>>(s, pow, ps, s0, out);
-    return launched();
+    constexpr int V = VEC<T>;
+    // 16-byte accesses need both parts of the array and every head's state on 16-byte boundaries
+    if (s.n_scores() % V == 0 && int64_t(s.dk) * s.dv % V == 0 && al16(ps) && al16(s0) && al16(out))
+        return launch_carry<T, V>(s, pow, ps, s0, out, st);
+    return launch_carry<T, 1>(s, pow, ps, s0, out, st);
 }
 
 template <typename T>
@@ -532,12 +675,26 @@ int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
     return launched();
 }
 
+template <typename T, int V>
+static int launch_step(const LaShape &s, const LaStepArgs<T> &a, cudaStream_t st)
+{
+    // whole rows of up to 32 x V columns per block; fewer where that leaves SMs idle
+    int cx = 32;
+    while (cx > 8 && (s.dv <= cx / 2 * V || s.bh() * ((s.dv + cx * V - 1) / (cx * V)) < 2 * 148)) cx /= 2;
+    const int slabs = (s.dv + cx * V - 1) / (cx * V);
+    DDG_CHECK(s.bh() * slabs <= 0x7fffffff, DDG_ERR_ARG, "linear attention: %lld heads are too many for one call",
+              (long long)s.bh());
+    k_la_step<T, V><<<unsigned(s.bh() * slabs), LA_THREADS, 0, st>>>(s, a, cx, slabs);
+    return launched();
+}
+
 template <typename T>
 int la_step(const LaShape &s, const LaStepArgs<T> &a, cudaStream_t st)
 {
     if (!s.bh()) return DDG_OK;
-    k_la_step<T><<<la_grid(s.n_step()), LA_THREADS, 0, st>>>(s, a);
-    return launched();
+    constexpr int V = VEC<T>;
+    if (s.dv % V == 0 && al16(a.s) && al16(a.s_ms) && al16(a.z) && al16(a.out)) return launch_step<T, V>(s, a, st);
+    return launch_step<T, 1>(s, a, st);
 }
 
 template <typename T>
