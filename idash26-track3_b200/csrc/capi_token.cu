@@ -16,6 +16,7 @@ int check_q4(const ddg_q4_weights *w)
     DDG_CHECK(w->group > 0 && w->group % 32 == 0, DDG_ERR_ARG, "group must be a multiple of 32 (got %d)", w->group);
     DDG_CHECK(w->K == 0 || w->N == 0 || (w->d_q && w->d_step), DDG_ERR_ARG, "null pointer");
     DDG_CHECK((reinterpret_cast<uintptr_t>(w->d_q) & 15) == 0, DDG_ERR_ARG, "4-bit codes must be 16-byte aligned");
+    DDG_CHECK((reinterpret_cast<uintptr_t>(w->d_step) & 3) == 0, DDG_ERR_ARG, "4-bit steps must be 4-byte aligned");
     return DDG_OK;
 }
 

@@ -14,17 +14,19 @@
 //
 // k_q4_tc, for more rows: the weights are 16-bit numbers, W + 2^15 = w0 + 2^8 w1
 // with unsigned bytes, and x = sum_l 2^(8l) x_l, so
-//   x . W = sum_s 2^(8s) (x_s . w0 + x_{s-1} . w1) - 2^15 sum_k x_k .
-// The weights are the M side of the MMA (128 outputs), and the limbs of MT
-// rows of x its N side (limb-major, P * MT columns): one MMA with w0 covers
-// every limb, one with w1 into the columns of the next limb every shifted one.
-// 2 wide MMAs per 32 k, and 2 P byte products where full-width ring weights
-// take P(P+1)/2.  Codes are expanded by all threads while the MMAs of earlier
-// stages run; the sums of a split K meet in the cluster's shared memory.
+//   x . W = sum_s 2^(8s) sum_k (w0 x_s + w1 x_{s-1})  -  2^15 sum_k x_k .
+// The weights are the M side of the MMA (128 outputs) as they are, two bytes a
+// weight; the N side has a row (x_s, x_{s-1}) per k for every limb s of MT rows
+// of x (limb-major, P * MT columns).  So a weight costs one multiply-add for
+// two of them and no byte shuffles, one MMA of 32 bytes covers 16 k of every
+// limb, and the whole product takes 2 P byte products where full-width ring
+// weights take P(P+1)/2.  One warp loads codes and x with TMA, one issues the
+// MMAs, the others expand codes and split x.  The sums of a split K meet in the
+// cluster's shared memory.
 #include <type_traits>
 
+#include "tma.cuh"
 #include "token.cuh"
-#include "umma.cuh"
 
 namespace ddg {
 
@@ -35,7 +37,8 @@ constexpr int Q4_THREADS = 256;
 // ------------------------------------------------------------------ one or two rows
 
 constexpr int GV_WARPS = Q4_THREADS / 32;
-constexpr int GV_R = 4;                       // outputs per lane group and pass
+template <typename T>
+constexpr int GV_R = sizeof(T) == 4 ? 4 : 2;  // outputs per lane group and pass (registers: P limb sums each)
 constexpr uint64_t GV_SMEM_MAX = 96 * 1024;
 
 // units of 32 k; a group of L lanes takes one unit each, KS warps of the CTA split the units
@@ -43,7 +46,7 @@ struct GvGeom {
     int U, L, nseg, KS, slots, blocks;
 };
 
-inline GvGeom gv_geom(int K, int N)
+inline GvGeom gv_geom(int K, int N, int R)
 {
     GvGeom g;
     g.U = (K + 31) / 32;
@@ -52,22 +55,22 @@ inline GvGeom gv_geom(int K, int N)
     g.nseg = (g.U + g.L - 1) / g.L;
     g.KS = g.nseg < 1 ? 1 : g.nseg < GV_WARPS ? g.nseg : GV_WARPS;
     g.slots = GV_WARPS / g.KS * (32 / g.L);
-    g.blocks = (N + g.slots * GV_R - 1) / (g.slots * GV_R);
+    g.blocks = (N + g.slots * R - 1) / (g.slots * R);
     return g;
 }
 
 template <typename T>
 uint64_t gv_smem(const GvGeom &g, int rows)
 {
-    return uint64_t(rows) * g.U * (32 * sizeof(T) + sizeof(T)) + uint64_t(GV_WARPS) * 32 * GV_R * rows * sizeof(T);
+    return uint64_t(rows) * g.U * (32 * sizeof(T) + sizeof(T)) + uint64_t(GV_WARPS) * 32 * GV_R<T> * rows * sizeof(T);
 }
 
 template <typename T, int MR>
-__global__ void __launch_bounds__(Q4_THREADS)
-    k_q4_gemv(const __grid_constant__ Q4Args<T> a, const __grid_constant__ GvGeom g, int64_t row_bytes)
+__global__ void __launch_bounds__(Q4_THREADS, 2)
+    k_q4_gemv(const __grid_constant__ Q4Args<T> a, const __grid_constant__ GvGeom g, int64_t row_bytes, int vec)
 {
-    constexpr int P = int(sizeof(T)), R = GV_R;
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    constexpr int P = int(sizeof(T)), R = GV_R<T>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint4 *const xs = reinterpret_cast<uint4 *>(smem_raw);                   // [MR][2P][U]
     T *const xsum8 = reinterpret_cast<T *>(xs + size_t(MR) * 2 * P * g.U);  // [MR][U]: 8 * sum of the unit's x
     T *const red = xsum8 + MR * g.U;                                        // [warp][lane group][R][MR]
@@ -103,12 +106,18 @@ __global__ void __launch_bounds__(Q4_THREADS)
         const int i = in ? i0 + lane : 0;
         const int m = i / (g.U * 4), u = (i >> 2) % g.U, j = i & 3;
         T e[8], sum = 0;
+        const int k0 = u * 32 + j * 8;
+        const T *const xp = a.x + int64_t(m) * a.ldx + k0;
+        if (in && vec && k0 + 8 <= a.w.K) {
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-            const int k = u * 32 + j * 8 + t;
-            e[t] = in && k < a.w.K ? __ldg(a.x + int64_t(m) * a.ldx + k) : T(0);
-            sum += e[t];
+            for (int t = 0; t < P / 2; t++)
+                *reinterpret_cast<uint4 *>(e + t * (16 / P)) = __ldg(reinterpret_cast<const uint4 *>(xp) + t);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 8; t++) e[t] = in && k0 + t < a.w.K ? __ldg(xp + t) : T(0);
         }
+#pragma unroll
+        for (int t = 0; t < 8; t++) sum += e[t];
         if (in) {
 #pragma unroll
             for (int par = 0; par < 2; par++) {
@@ -208,25 +217,41 @@ __global__ void __launch_bounds__(Q4_THREADS)
 
 // ------------------------------------------------------------------ more rows: tensor cores
 
-constexpr int QT_KC = 64;     // k per stage (two MMA K-steps)
-constexpr int QT_STAGES = 3;
-constexpr int QT_MAX_CHUNKS = 32768 / QT_KC;
-constexpr uint32_t QT_PLANE = TC_BM * 32;  // bytes of one weight plane per K-step
+constexpr int QT_STAGES = 2;
+constexpr int QT_MAX_K = 32768;            // k per CTA: a column's sum, 2 * 255^2 * K, stays below 2^32
+// operands lie in 16-byte chunks of 8 k, chunk-major: rows 16 bytes apart,
+// chunks of A 2048 and of B 16 NB + 16 bytes apart (the pad spreads the chunks
+// of one row, written by neighbouring lanes, over the banks)
+constexpr uint32_t QT_A_CHUNK = TC_BM * 16;
 
-template <typename T, int MT>
+// MT rows of x per CTA and NA 128-output weight tiles, which share the split of x
+template <typename T, int MT, int NA>
 struct QtShape {
     static constexpr int P = int(sizeof(T));
-    static constexpr int NB = P * MT;                              // columns of the w0 MMA
-    static constexpr int NH = ((P - 1) * MT + 15) / 16 * 16;       // columns of the w1 MMA (from column MT)
-    static constexpr int COLS = tmem_cols(NB > MT + NH ? NB : MT + NH);
-    static constexpr uint32_t B_STEP = NB * 32;                    // bytes of the x limbs per K-step
-    static constexpr uint32_t A_STAGE = 2 * 2 * QT_PLANE, STAGE = A_STAGE + 2 * B_STEP;
-    static constexpr int EK = 64 / P;                              // k per x item (64 bytes)
-    static constexpr int ITEMS = MT * (QT_KC / EK);
-    // [barriers, TMEM address | sums of x | pad to 1024 | stages | slack]
-    static constexpr uint32_t HEAD = 64 + MT * P;
-    static constexpr uint32_t SMEM = HEAD + 1024 + QT_STAGES * STAGE + 4096;
-    static_assert(NB % 16 == 0 && NB <= 256 && ITEMS <= Q4_THREADS, "tile");
+    static constexpr int THREADS = NA * Q4_THREADS;                // splitting threads, before the MMA warp
+    static constexpr int NB = P * MT;                              // MMA columns
+    // k per stage: narrow MMAs are issue-bound (a commit takes as long as five
+    // of them), so they get twice the K per commit and the SM to themselves
+    static constexpr int KC = NB <= 64 ? 128 : 64, UPT = KC / 64, CTAS = NB == 128 ? 2 : 1;
+    static constexpr int CH = KC / 8, XROW = KC / 8;               // chunks per stage; x items of 8 k per row
+    static constexpr int COLS = tmem_cols(NA * NB);
+    static constexpr uint32_t B_CHUNK = NB * 16 + 16;
+    static constexpr uint32_t A_TILE = CH * QT_A_CHUNK, A_STAGE = NA * A_TILE, STAGE = A_STAGE + CH * B_CHUNK;
+    static constexpr int ITEMS = MT * XROW, XPT = (ITEMS + THREADS - 1) / THREADS;
+    // A stage's codes (UPT boxes of 32 bytes a row), x and steps as they lie in
+    // memory, loaded RD stages ahead: the memory needs about 40 KB of codes in
+    // flight per SM for its latency.  (Asynchronous 16-byte copies by the
+    // expanding threads took 600-1000 cycles a stage to issue.)
+    static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = UPT * RAW_BOX, RAW_STEPS = RAW_X + MT * KC * P;
+    static constexpr uint32_t RAW = RAW_STEPS + THREADS * UPT * 4;
+    static constexpr int RD_FIT = int(((CTAS == 2 ? 106 : 212) * 1024 - QT_STAGES * STAGE) / RAW);
+    static constexpr int RD = RD_FIT < 2 ? 2 : RD_FIT > 8 ? 8 : RD_FIT;
+    // [barriers, TMEM address | sums of x | pad to 1024 | stages | raw stages | slack]
+    static constexpr uint32_t HEAD = 256 + MT * P;
+    static constexpr uint32_t XPITCH = (ITEMS < THREADS ? ITEMS : THREADS) * 16;  // between 16-byte pieces of the x items
+    static constexpr uint32_t SMEM = HEAD + 1024 + QT_STAGES * STAGE + RD * RAW + 2048;
+    static_assert(NB % 16 == 0 && NB <= 256 && STAGE % 128 == 0 && RAW % 128 == 0 && RAW_X % 128 == 0, "tile");
+    static_assert(THREADS % XROW == 0 && (ITEMS % THREADS == 0 || XPT == 1), "x items");
 };
 
 __device__ __forceinline__ void cluster_sync()
@@ -251,33 +276,41 @@ __device__ __forceinline__ T ld_cluster(const T *p, uint32_t rank)
     }
 }
 
-// 8 codes times a step, plus 2^15: byte planes (low, high) of k = 0..3 and 4..7
-__device__ __forceinline__ void q4_expand(uint32_t c, uint32_t s, uint32_t bias, uint32_t &lo0, uint32_t &lo1,
-                                          uint32_t &hi0, uint32_t &hi1)
+// 8 codes times a step, plus 2^15, as 16-bit weights in the order k = 0 4 1 5 2 6 3 7
+__device__ __forceinline__ uint4 q4_expand(uint32_t c, uint32_t s, uint32_t bias)
 {
-    // codes k and k + 4 in the two halves of a word: one multiply-add makes both 16-bit weights (no
-    // carry between the halves: 0 <= s * code + 2^15 - 8 s < 2^16 for s <= 4095)
-    uint32_t p[4];
-    byte_planes((c & 0x000f000fu) * s + bias, ((c >> 4) & 0x000f000fu) * s + bias, ((c >> 8) & 0x000f000fu) * s + bias,
-                ((c >> 12) & 0x000f000fu) * s + bias, p);
-    lo0 = p[0], hi0 = p[1], lo1 = p[2], hi1 = p[3];
+    // codes k and k + 4 in the two halves of a word: one multiply-add makes both weights (no carry
+    // between the halves: 0 <= s * code + 2^15 - 8 s < 2^16 for s <= 4095)
+    return make_uint4((c & 0x000f000fu) * s + bias, ((c >> 4) & 0x000f000fu) * s + bias,
+                      ((c >> 8) & 0x000f000fu) * s + bias, ((c >> 12) & 0x000f000fu) * s + bias);
 }
 
-template <typename T, int MT>
-__global__ void __launch_bounds__(Q4_THREADS, 2)
-    k_q4_tc(const __grid_constant__ Q4Args<T> a, int64_t row_bytes, int per, int vec, uint32_t *err)
+// bytes (s, s - 1) of a, then of b
+__device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int s)
 {
-    using S = QtShape<T, MT>;
-    constexpr int P = S::P;
+    return s == 0 ? __byte_perm(a, b, 0x0400) & 0x00ff00ffu
+                  : __byte_perm(a, b, uint32_t(s | (s - 1) << 4 | (s + 4) << 8 | (s + 3) << 12));
+}
+
+template <typename T, int MT, int NA>
+__global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
+    k_q4_tc(const __grid_constant__ Q4Args<T> a, const __grid_constant__ CUtensorMap codes_map,
+            const __grid_constant__ CUtensorMap x_map, int per, int vec, uint32_t group_magic, uint32_t *err)
+{
+    using S = QtShape<T, MT, NA>;
+    constexpr int P = S::P, THREADS = S::THREADS, KC = S::KC, WARPS = THREADS / 32;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint64_t *const bars = reinterpret_cast<uint64_t *>(smem_raw);
-    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem_raw + 32);
-    T *const xsum = reinterpret_cast<T *>(smem_raw + 64);  // [MT]
+    uint64_t *const empty = reinterpret_cast<uint64_t *>(smem_raw), *const full = empty + QT_STAGES;
+    uint64_t *const raw_full = full + QT_STAGES, *const raw_empty = raw_full + 8;  // (2 + 2 + 8 + 8) x 8 bytes
+    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem_raw + 192);
+    T *const xsum = reinterpret_cast<T *>(smem_raw + 256);  // [MT]
     uint8_t *const smem = smem_raw + S::HEAD + ((1024u - ((smem_addr(smem_raw) + S::HEAD) & 1023u)) & 1023u);
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n0 = blockIdx.x * TC_BM, m0 = blockIdx.y * MT;
-    const int nkc = (a.w.K + QT_KC - 1) / QT_KC, c0 = blockIdx.z * per;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const bool mma_warp = warp == WARPS, tma_warp = warp == WARPS + 1, expands = warp < WARPS;
+    const int half = expands ? warp >> 3 : 0;  // this thread's weight tile
+    const int n0 = (blockIdx.x * NA + half) * TC_BM, m0 = blockIdx.y * MT;
+    const int nkc = (a.w.K + KC - 1) / KC, c0 = blockIdx.z * per;
     const int nk = nkc - c0 < per ? (nkc - c0 > 0 ? nkc - c0 : 0) : per;
 
     if (warp == 0) {
@@ -287,7 +320,8 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < QT_STAGES; i++) mbar_init(bars + i, 1);
+        for (int i = 0; i < QT_STAGES; i++) mbar_init(empty + i, 1), mbar_init(full + i, WARPS);
+        for (int i = 0; i < S::RD; i++) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid < MT) xsum[tid] = 0;
@@ -296,197 +330,261 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // this thread's unit of codes (row, 32 k) and item of x (row, EK k) of every stage
-    const int arow = 16 * warp + (lane & 15), aun = lane >> 4;
-    const int xm = tid % MT, xk = tid / MT;
-    const bool has_x = tid < S::ITEMS, xrow = has_x && m0 + xm < a.M;
-    const uint4 *const crow = reinterpret_cast<const uint4 *>(a.w.q + int64_t(n0 + arow) * row_bytes);
+    // this thread's units of codes (row, 32 k each) and items of x (row, 8 k each) of every stage
+    const int arow = 16 * (warp & 7) + (lane & 15), aun = lane >> 4;  // units aun, aun + 2
+    const int xk = tid % S::XROW * 8, xm = tid / S::XROW;
+    const bool has_x = expands && tid < S::ITEMS;
     const int units = (a.w.K + 31) / 32;
-    const bool arow_ok = n0 + arow < a.w.N;
-    const T *const xptr = a.x + int64_t(m0 + xm) * a.ldx;
-    T sum = 0;
-    uint4 code;
-    uint32_t step;
-    T xe[S::EK];
-
-    auto load_stage = [&](int c) {
-        const int u = 2 * c + aun;
-        code = make_uint4(0, 0, 0, 0), step = 0;
-        if (arow_ok && u < units) {
-            code = __ldg(crow + u);
-            step = __ldg(a.w.step + int64_t(u * 32 / a.w.group) * a.w.N + n0 + arow) & Q4_STEP_MAX;
-        }
-        const int k = c * QT_KC + xk * S::EK;
-        if (xrow && vec && k + S::EK <= a.w.K) {
-            const uint4 *v = reinterpret_cast<const uint4 *>(xptr + k);
+    T sum[S::XPT];
 #pragma unroll
-            for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(xe + i * (16 / P)) = __ldg(v + i);
-        } else {
-#pragma unroll
-            for (int i = 0; i < S::EK; i++) xe[i] = xrow && k + i < a.w.K ? __ldg(xptr + k + i) : T(0);
-        }
+    for (int i = 0; i < S::XPT; i++) sum[i] = 0;
+    uint8_t *const raw = smem + QT_STAGES * S::STAGE;
+    const uint32_t raw_steps = smem_addr(raw) + S::RAW_STEPS + 4 * tid, raw_x = smem_addr(raw) + S::RAW_X + 16 * tid;
+    // index of the step of unit u of a row: u / (group / 32), by the exact reciprocal (u < 2^13)
+    auto step_at = [&](int u) {
+        return int64_t(group_magic ? __umulhi(uint32_t(u), group_magic) : uint32_t(u)) * a.w.N + n0 + arow;
     };
-    auto store_stage = [&](int st) {
-        uint8_t *const base = smem + st * S::STAGE;
-        const uint32_t bias = (0x8000u - 8u * step) * 0x10001u;
-        const uint32_t cw[4] = {code.x, code.y, code.z, code.w};
-        uint8_t *const pa = base + aun * 2 * QT_PLANE + (arow >> 3) * 256 + (arow & 7) * 16;
+    // copies stage c's steps into raw stage r (and x where its rows are not on 16-byte boundaries);
+    // what lies outside the matrices arrives as zeros
+    auto issue = [&](int c, int r) {
+        const uint32_t ro = uint32_t(r) * S::RAW;
 #pragma unroll
-        for (int hf = 0; hf < 2; hf++) {
-            uint4 lo, hi;
-            q4_expand(cw[2 * hf], step, bias, lo.x, lo.y, hi.x, hi.y);
-            q4_expand(cw[2 * hf + 1], step, bias, lo.z, lo.w, hi.z, hi.w);
-            *reinterpret_cast<uint4 *>(pa + hf * 128) = lo;
-            *reinterpret_cast<uint4 *>(pa + QT_PLANE + hf * 128) = hi;
+        for (int i = 0; i < S::UPT; i++) {
+            const int u = KC / 32 * c + aun + 2 * i;
+            const bool in = u < units && n0 + arow < a.w.N;
+            const int64_t at = in ? step_at(u) : 0;
+            // the aligned pair of steps that holds this one (only its own half at the array's end)
+            cp_async<4>(raw_steps + ro + i * THREADS * 4, a.w.step + (at & ~int64_t(1)), in ? (at & 1 ? 4 : 2) : 0);
+        }
+        if (has_x && !vec) {
+#pragma unroll
+            for (int j = 0; j < S::XPT; j++) {
+                const int m = xm + j * (THREADS / S::XROW), k = c * KC + xk;
+                const T *const xp = a.x + int64_t(m0 + m) * a.ldx + k;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const bool in = m0 + m < a.M && k + i < a.w.K;
+                    cp_async<P>(raw_x + ro + j * THREADS * 8 * P + i / (16 / P) * S::XPITCH + i % (16 / P) * P,
+                                in ? xp + i : a.x, in ? P : 0);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+    // expands raw stage r into the planes of stage st
+    auto store_stage = [&](int c, int r, int st) {
+        uint8_t *const base = smem + st * S::STAGE;
+        const uint8_t *const rp = raw + uint32_t(r) * S::RAW;
+#pragma unroll
+        for (int i = 0; i < S::UPT; i++) {
+            const uint4 code =
+                *reinterpret_cast<const uint4 *>(rp + i * S::RAW_BOX + (half * TC_BM + arow) * 32 + aun * 16);
+            const uint32_t odd = uint32_t(step_at(KC / 32 * c + aun + 2 * i)) & 1;
+            const uint32_t step =
+                (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + (i * THREADS + tid) * 4) >> (16 * odd)) & Q4_STEP_MAX;
+            const uint32_t bias = (0x8000u - 8u * step) * 0x10001u;
+            uint8_t *const pa = base + half * S::A_TILE + (aun + 2 * i) * 4 * QT_A_CHUNK + arow * 16;
+            *reinterpret_cast<uint4 *>(pa) = q4_expand(code.x, step, bias);
+            *reinterpret_cast<uint4 *>(pa + QT_A_CHUNK) = q4_expand(code.y, step, bias);
+            *reinterpret_cast<uint4 *>(pa + 2 * QT_A_CHUNK) = q4_expand(code.z, step, bias);
+            *reinterpret_cast<uint4 *>(pa + 3 * QT_A_CHUNK) = q4_expand(code.w, step, bias);
         }
         if (has_x) {
 #pragma unroll
-            for (int i = 0; i < S::EK; i++) sum += xe[i];
-            const int k = xk * S::EK;  // within the stage
-            uint8_t *const pb = base + S::A_STAGE + (k >> 5) * S::B_STEP + ((k >> 4) & 1) * 128 + (k & 15);
-            uint32_t w[P][S::EK / 4];
+            for (int j = 0; j < S::XPT; j++) {
+                T xe[8];
 #pragma unroll
-            for (int i = 0; i < S::EK / 4; i++) {
-                uint32_t p[4];
-                byte_planes(uint32_t(xe[4 * i]), uint32_t(xe[4 * i + 1]), uint32_t(xe[4 * i + 2]),
-                            uint32_t(xe[4 * i + 3]), p);
+                for (int i = 0; i < P / 2; i++)
+                    *reinterpret_cast<uint4 *>(xe + i * (16 / P)) = *reinterpret_cast<const uint4 *>(
+                        rp + S::RAW_X +
+                        (vec ? uint32_t((xm + j * (THREADS / S::XROW)) * KC + xk) * P + i * 16
+                             : j * THREADS * 8 * P + i * S::XPITCH + tid * 16));
 #pragma unroll
-                for (int l = 0; l < 4; l++) w[l][i] = p[l];
-                if constexpr (P == 8) {
-                    byte_planes(uint32_t(uint64_t(xe[4 * i]) >> 32), uint32_t(uint64_t(xe[4 * i + 1]) >> 32),
-                                uint32_t(uint64_t(xe[4 * i + 2]) >> 32), uint32_t(uint64_t(xe[4 * i + 3]) >> 32), p);
+                for (int i = 0; i < 8; i++) sum[j] += xe[i];
+                uint8_t *const pb = base + S::A_STAGE + (xk >> 3) * S::B_CHUNK + (xm + j * (THREADS / S::XROW)) * 16;
 #pragma unroll
-                    for (int l = 0; l < 4; l++) w[4 + l][i] = p[l];
+                for (int l = 0; l < P; l++) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t lo0 = uint32_t(xe[i]), lo1 = uint32_t(xe[i + 4]);
+                        if constexpr (P == 4) {
+                            w[i] = byte_pair(lo0, lo1, l);
+                        } else {
+                            const uint32_t hi0 = uint32_t(uint64_t(xe[i]) >> 32), hi1 = uint32_t(uint64_t(xe[i + 4]) >> 32);
+                            if (l < 4)
+                                w[i] = byte_pair(lo0, lo1, l);
+                            else if (l < 7)  // bytes 3..6 of x
+                                w[i] = byte_pair(__funnelshift_l(lo0, hi0, 8), __funnelshift_l(lo1, hi1, 8), l - 3);
+                            else
+                                w[i] = byte_pair(hi0, hi1, 3);
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(pb + l * MT * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-            }
-#pragma unroll
-            for (int l = 0; l < P; l++) {
-                const int row = l * MT + xm;
-                uint8_t *const d = pb + (row >> 3) * 256 + (row & 7) * 16;
-                if constexpr (P == 4)
-                    *reinterpret_cast<uint4 *>(d) = make_uint4(w[l][0], w[l][1], w[l][2], w[l][3]);
-                else
-                    *reinterpret_cast<uint2 *>(d) = make_uint2(w[l][0], w[l][1]);
             }
         }
     };
 
-    constexpr uint32_t ID0 = i8_idesc(S::NB, false), ID1 = i8_idesc(S::NH, false);
+    constexpr uint32_t IDESC = i8_idesc(S::NB, false);
     bool ok = true;
-    if (nk > 0) load_stage(c0);
-    for (int c = 0; c < nk; c++) {
-        const int st = c % QT_STAGES;
-        bool mine = true;
-        if (c >= QT_STAGES) mine = mbar_wait(&bars[st], uint32_t((c / QT_STAGES - 1) & 1));
-        if (mine) store_stage(st);
-        if (c + 1 < nk) load_stage(c0 + c + 1);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        // CTA-uniform: every thread leaves the loop together if any wait gave up
-        if (!__syncthreads_and(mine ? 1 : 0)) {
-            ok = false;
-            break;
-        }
-        if (tid == 0) {
+    if (mma_warp) {
+        const bool leader = elect_one();
+        for (int c = 0; c < nk && ok; c++) {
+            const int st = c % QT_STAGES;
+            ok = mbar_wait(&full[st], uint32_t((c / QT_STAGES) & 1));
             tc_fence_after();
-            const uint32_t sa = smem_addr(smem + st * S::STAGE), sb = sa + S::A_STAGE;
+            if (ok && leader) {
+                const uint32_t sa = smem_addr(smem + st * S::STAGE), sb = sa + S::A_STAGE;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint64_t db = smem_desc(sb + h * S::B_STEP, 128, 256);
-                mma_i8(tmem, smem_desc(sa + h * 2 * QT_PLANE, 128, 256), db, ID0, (c > 0 || h > 0) ? 1u : 0u);
-                // columns past limb P-1 collect products of 2^(8P) and above, which nobody reads
-                mma_i8(tmem + MT, smem_desc(sa + (h * 2 + 1) * QT_PLANE, 128, 256), db, ID1, 1u);
+                for (int h = 0; h < KC / 16; h++) {
+                    const uint64_t db = smem_desc(sb + h * 2 * S::B_CHUNK, S::B_CHUNK, 128);
+#pragma unroll
+                    for (int t = 0; t < NA; t++)
+                        mma_i8(tmem + t * S::NB, smem_desc(sa + t * S::A_TILE + h * 2 * QT_A_CHUNK, QT_A_CHUNK, 128), db,
+                               IDESC, (c > 0 || h > 0) ? 1u : 0u);
+                }
+                mma_commit(&empty[st]);
             }
-            mma_commit(&bars[st]);
+            __syncwarp();
         }
+    } else if (tma_warp) {
+        const bool leader = elect_one();
+        for (int c = 0, r = 0; c < nk && ok; c++, r = r + 1 == S::RD ? 0 : r + 1) {
+            if (c >= S::RD) ok = mbar_wait(&raw_empty[r], uint32_t((c / S::RD - 1) & 1));
+            if (ok && leader) {
+                const uint32_t ra = smem_addr(raw) + uint32_t(r) * S::RAW;
+                mbar_expect(&raw_full[r], S::UPT * S::RAW_BOX + (vec ? MT * KC * P : 0));
+#pragma unroll
+                for (int i = 0; i < S::UPT; i++)
+                    tma_load_2d(ra + i * S::RAW_BOX, &codes_map, (c0 + c) * (KC / 2) + 32 * i, n0, &raw_full[r]);
+                if (vec) tma_load_2d(ra + S::RAW_X, &x_map, (c0 + c) * KC, m0, &raw_full[r]);
+            }
+            __syncwarp();
+        }
+        // nobody leaves with copies in flight
+        if (ok && nk > 0) ok = mbar_wait(&raw_full[(nk - 1) % S::RD], uint32_t(((nk - 1) / S::RD) & 1));
+    } else {
+        for (int c = 0; c < S::RD; c++) {
+            if (c < nk)
+                issue(c0 + c, c);
+            else
+                cp_async_commit();
+        }
+        for (int c = 0, r = 0; c < nk; c++, r = r + 1 == S::RD ? 0 : r + 1) {
+            const int st = c % QT_STAGES;
+            cp_async_wait<S::RD - 1>();  // this thread's copies of stage c have landed
+            ok = mbar_wait(&raw_full[r], uint32_t((c / S::RD) & 1));
+            if (ok && c >= QT_STAGES) ok = mbar_wait(&empty[st], uint32_t((c / QT_STAGES - 1) & 1));
+            if (!__all_sync(0xffffffffu, ok)) break;
+            store_stage(c0 + c, r, st);
+            if (c + S::RD < nk)
+                issue(c0 + c + S::RD, r);
+            else
+                cp_async_commit();
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]), mbar_arrive(&raw_empty[r]);
+        }
+        cp_async_wait<0>();
     }
-    if (ok && nk > 0) ok = mbar_wait(&bars[(nk - 1) % QT_STAGES], uint32_t(((nk - 1) / QT_STAGES) & 1));
-    if (has_x) atomicAdd(reinterpret_cast<std::conditional_t<P == 4, unsigned int, unsigned long long> *>(xsum + xm), sum);
+    // the last stage's commit covers every MMA before it
+    if (ok && nk > 0) ok = mbar_wait(&empty[(nk - 1) % QT_STAGES], uint32_t(((nk - 1) / QT_STAGES) & 1));
+    if (has_x) {
+        using U = std::conditional_t<P == 4, unsigned int, unsigned long long>;
+#pragma unroll
+        for (int j = 0; j < S::XPT; j++) atomicAdd(reinterpret_cast<U *>(xsum + xm + j * (THREADS / S::XROW)), U(sum[j]));
+    }
     const int all_ok = __syncthreads_and(ok ? 1 : 0);
     tc_fence_after();
 
-    // out += or hand over: this CTA's sum of (row m, output n0 + 32 q + lane)
-    const bool split = gridDim.z > 1;
-    T *const part = reinterpret_cast<T *>(smem);  // [MT][128], the stages are done
-    const int q = warp & 3, h = warp >> 2, nl = 32 * q + lane;
-    auto give = [&](int m, T v) {
-        if (nk > 0)
-            v -= xsum[m] << 15;
-        else
-            v = 0;
-        if (split) {
-            part[m * TC_BM + nl] = v;
-        } else if (n0 + nl < a.w.N && m0 + m < a.M) {
-            const int64_t e = int64_t(m0 + m) * a.w.N + n0 + nl;
-            v *= a.sign;
-            if (a.bias) v += __ldg(a.bias + n0 + nl);
-            if (a.Add) v += a.Add[e];
-            a.out[e] = v;
-        }
-    };
-    if (all_ok) {
-        const uint32_t lanes = tmem + (uint32_t(32 * q) << 16);
-        if constexpr (MT >= 16) {
+    // this CTA's sums of (row m, output n) to shared memory (the stages are done), all of them added up
+    // over the cluster and written in batches whose loads overlap
+    T *const part = reinterpret_cast<T *>(smem);  // [MT][NA * 128]
+    constexpr int PITCH = NA * TC_BM;
+    if (all_ok && expands) {
+        const int q = warp & 3, h = (warp >> 2) & 1, nl = half * TC_BM + 32 * q + lane;
+        const uint32_t lanes = tmem + half * S::NB + (uint32_t(32 * q) << 16);
+        constexpr int CW = MT < 8 ? MT : 8, STEP = MT < 16 ? CW : 2 * CW;  // rows per TMEM pass; narrow tiles: warps 0-3
+        if (MT >= 16 || h == 0) {
 #pragma unroll 1
-            for (int m = h * (MT / 2); m < (h + 1) * (MT / 2); m += 8) {
-                T r[8];
+            for (int m = MT < 16 ? 0 : h * CW; m < MT; m += STEP) {
+                uint32_t v[P][8];
+                if constexpr (MT >= 8) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) r[e] = 0;
+                    for (int s = 0; s < P; s++) tmem_ld8(lanes + s * MT + m, v[s]);
+                } else {
+                    // MT = 4 or 2: eight columns hold 8 / MT limbs
+                    uint32_t t[S::NB / 8][8];
 #pragma unroll
-                for (int s = 0; s < P; s++) {
-                    uint32_t v[8];
-                    tmem_ld8(lanes + s * MT + m, v);
+                    for (int i = 0; i < S::NB / 8; i++) tmem_ld8(lanes + 8 * i, t[i]);
                     tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 8; e++) r[e] += T(v[e]) << (8 * s);
+                    for (int s = 0; s < P; s++)
+#pragma unroll
+                        for (int e = 0; e < CW; e++) v[s][e] = t[(s * MT + e) / 8][(s * MT + e) % 8];
                 }
-#pragma unroll
-                for (int e = 0; e < 8; e++) give(m + e, r[e]);
-            }
-        } else if (h == 0) {
-            uint32_t v[S::NB];
-#pragma unroll
-            for (int i = 0; i < S::NB; i += 8) {
-                uint32_t t[8];
-                tmem_ld8(lanes + i, t);
                 tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[i + e] = t[e];
-            }
+                for (int e = 0; e < CW; e++) {
+                    T r = T(0) - (xsum[m + e] << 15);
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-                T r = 0;
-#pragma unroll
-                for (int s = 0; s < P; s++) r += T(v[s * MT + m]) << (8 * s);
-                give(m, r);
+                    for (int s = 0; s < P; s++) r += T(v[s][e]) << (8 * s);
+                    part[(m + e) * PITCH + nl] = nk > 0 ? r : T(0);  // a split's last CTA may have no stage
+                }
             }
         }
-    } else if (tid == 0) {
-        atomicOr(err, 4u);
     }
+    if (!all_ok && tid == 0) atomicOr(err, 4u);
     tc_fence_before();
-    if (split) {
+    const bool split = gridDim.z > 1;
+    if (split)
         cluster_sync();
-        const int S_ = gridDim.z, rank = blockIdx.z;
-        const int rows = a.M - m0 < MT ? a.M - m0 : MT;
-        for (int i = rank * Q4_THREADS + tid; i < rows * TC_BM; i += S_ * Q4_THREADS) {
-            const int m = i / TC_BM, n = n0 + i % TC_BM;
-            if (n >= a.w.N) continue;
-            T v = 0;
-            for (int z = 0; z < S_; z++) v += ld_cluster(part + i, z);
-            const int64_t e = int64_t(m0 + m) * a.w.N + n;
-            v *= a.sign;
-            if (a.bias) v += __ldg(a.bias + n);
-            if (a.Add) v += a.Add[e];
-            a.out[e] = v;
-        }
-        cluster_sync();  // nobody leaves while its sums are read
-    } else {
+    else
         __syncthreads();
+    if (expands && all_ok) {
+        const int parts = int(gridDim.z), rank = int(blockIdx.z);
+        const int nl = tid % PITCH, n = blockIdx.x * PITCH + nl;
+        constexpr int ROWS = THREADS / PITCH, U = 8;  // rows per pass; passes per batch
+        if (n < a.w.N) {
+            const T bias = a.bias ? __ldg(a.bias + n) : T(0);
+            for (int mb = rank * ROWS + tid / PITCH; mb < MT; mb += U * ROWS * parts) {
+                T add[U], v[U];
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    const int m = mb + i * ROWS * parts;
+                    const bool in = m < MT && m0 + m < a.M;
+                    add[i] = in && a.Add ? a.Add[int64_t(m0 + m) * a.w.N + n] : T(0);
+                    v[i] = 0;
+                    if (in) {
+                        if (parts == 1)
+                            v[i] = part[m * PITCH + nl];
+                        else
+                            for (int z = 0; z < parts; z++) v[i] += ld_cluster(part + m * PITCH + nl, z);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    const int m = mb + i * ROWS * parts;
+                    if (m < MT && m0 + m < a.M) a.out[int64_t(m0 + m) * a.w.N + n] = a.sign * v[i] + bias + add[i];
+                }
+            }
+        }
     }
+    if (split) cluster_sync();  // nobody leaves while its sums are read
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");
     }
+}
+
+// an empty sum: out = bias + Add
+template <typename T>
+__global__ void __launch_bounds__(Q4_THREADS) k_q4_empty(const __grid_constant__ Q4Args<T> a)
+{
+    const int64_t n = int64_t(a.M) * a.w.N;
+    for (int64_t e = int64_t(blockIdx.x) * Q4_THREADS + threadIdx.x; e < n; e += int64_t(gridDim.x) * Q4_THREADS)
+        a.out[e] = (a.bias ? a.bias[e % a.w.N] : T(0)) + (a.Add ? a.Add[e] : T(0));
 }
 
 // one group of one output per thread: the smallest step whose codes -7..7
@@ -540,52 +638,66 @@ static int q4_smem_limit(K kern, uint64_t bytes, int (&configured)[64])
     return DDG_OK;
 }
 
+// 16-byte loads of x: its rows start on 16-byte boundaries
+template <typename T>
+static int q4_vec(const Q4Args<T> &a)
+{
+    return (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx * int64_t(sizeof(T)) % 16 == 0;
+}
+
 template <typename T, int MR>
 static int launch_gemv(const Q4Args<T> &a, cudaStream_t st)
 {
     static thread_local int configured[64];
     auto kern = k_q4_gemv<T, MR>;
-    const GvGeom g = gv_geom(a.w.K, a.w.N);
+    const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
     DDG_TRY(q4_smem_limit(kern, GV_SMEM_MAX, configured));
-    // up to three CTAs an SM, each splitting x once for all its outputs
-    const int grid = g.blocks < 3 * 148 ? g.blocks : 3 * 148;
-    kern<<<grid, Q4_THREADS, gv_smem<T>(g, MR), st>>>(a, g, int64_t(q4_row_bytes(a.w.K)));
+    // two CTAs an SM, each splitting x once for all its outputs
+    const int grid = g.blocks < 2 * 148 ? g.blocks : 2 * 148;
+    kern<<<grid, Q4_THREADS, gv_smem<T>(g, MR), st>>>(a, g, int64_t(q4_row_bytes(a.w.K)), q4_vec(a));
     note_launch();
     DDG_CUDA(cudaGetLastError());
     return DDG_OK;
 }
 
-template <typename T, int MT>
+template <typename T, int MT, int NA = 1>
 static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
 {
-    using S = QtShape<T, MT>;
+    using S = QtShape<T, MT, NA>;
     static thread_local int configured[64];
-    auto kern = k_q4_tc<T, MT>;
+    auto kern = k_q4_tc<T, MT, NA>;
     DDG_TRY(q4_smem_limit(kern, S::SMEM, configured));
     uint32_t *err = nullptr;
     DDG_TRY(ring_gemm_err_word(&err));
-    const int nkc = (a.w.K + QT_KC - 1) / QT_KC;
-    const int64_t gn = (int64_t(a.w.N) + TC_BM - 1) / TC_BM, gm = (int64_t(a.M) + MT - 1) / MT;
+    const int nkc = (a.w.K + S::KC - 1) / S::KC;
+    const int64_t gn = (int64_t(a.w.N) + NA * TC_BM - 1) / (NA * TC_BM), gm = (int64_t(a.M) + MT - 1) / MT;
     DDG_CHECK(gm <= 65535, DDG_ERR_ARG, "fc_q4: %d rows are too many for one call", a.M);
-    // K split over a cluster until two CTAs an SM are busy, two stages each at the least
+    // K split over a cluster while that leaves every CTA resident at once and two
+    // stages each.  Clusters of four: of eight, only 15 fit the device at a time
+    // (256 CTAs of a 4 x 4096 x 4096 product took three rounds).
     int split = 1;
-    while (split < 8 && gn * gm * split * 2 <= 2 * 148 && nkc >= 4 * split) split *= 2;
-    // a column's sum stays below 2^32: 2 * 255^2 * K per CTA, K <= 2^15
-    while (split < 8 && nkc > QT_MAX_CHUNKS * split) split *= 2;
-    DDG_CHECK(nkc <= QT_MAX_CHUNKS * split, DDG_ERR_ARG, "fc_q4: K = %d is too long (at most %d for %d rows)", a.w.K,
-              QT_MAX_CHUNKS * 8 * QT_KC, a.M);
+    while (NA == 1 && split < 4 && gn * gm * split * 2 <= S::CTAS * 148 && nkc >= 4 * split) split *= 2;
+    const int most = QT_MAX_K / S::KC;
+    while (NA == 1 && split < 8 && nkc > most * split) split *= 2;
+    DDG_CHECK(nkc <= most * split, DDG_ERR_ARG, "fc_q4: K = %d is too long (at most %d)", a.w.K, 8 * QT_MAX_K);
     const int per = nkc ? (nkc + split - 1) / split : 1;
-    const int vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.ldx * int64_t(sizeof(T)) % 16 == 0;
+    const int vec = q4_vec(a);
+    const uint32_t gd = uint32_t(a.w.group / 32);
+    const uint32_t magic = gd == 1 ? 0 : uint32_t((uint64_t(1) << 32) / gd + 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(gn), unsigned(gm), unsigned(split));
-    cfg.blockDim = dim3(Q4_THREADS);
+    cfg.blockDim = dim3(S::THREADS + 64);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 1, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = unsigned(split);
     cfg.attrs = at, cfg.numAttrs = 1;
-    DDG_CUDA(cudaLaunchKernelEx(&cfg, kern, a, int64_t(q4_row_bytes(a.w.K)), per, vec, err));
+    const uint64_t row_bytes = q4_row_bytes(a.w.K);
+    CUtensorMap codes_map, x_map = {};
+    DDG_TRY(tma_map_2d(&codes_map, a.w.q, 1, row_bytes, a.w.N, row_bytes, 32, NA * TC_BM));
+    if (vec) DDG_TRY(tma_map_2d(&x_map, a.x, sizeof(T), a.w.K, a.M, a.ldx * sizeof(T), S::KC, MT));
+    DDG_CUDA(cudaLaunchKernelEx(&cfg, kern, a, codes_map, x_map, per, vec, magic, err));
     note_launch();
     return DDG_OK;
 }
@@ -594,22 +706,32 @@ template <typename T>
 int fc_q4(const Q4Args<T> &a, cudaStream_t st)
 {
     if (int64_t(a.M) * a.w.N == 0) return DDG_OK;
-    const GvGeom g = gv_geom(a.w.K, a.w.N);
+    if (a.w.K == 0) {
+        k_q4_empty<T><<<148, Q4_THREADS, 0, st>>>(a);
+        note_launch();
+        DDG_CUDA(cudaGetLastError());
+        return DDG_OK;
+    }
+    const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
     if (a.M <= 2 && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
         return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
-    // the fewest rows per tile that hold them all, up to 256 MMA columns
+    // the fewest rows per tile that hold them all, up to 256 MMA columns; two
+    // weight tiles per CTA where those alone give every SM one (each split of x
+    // then serves 256 outputs), and K needs no split for the sums' range
+    constexpr int MT = 256 / int(sizeof(T));
+    const bool wide = (int64_t(a.w.N) + 255) / 256 * ((int64_t(a.M) + MT - 1) / MT) >= 148 && a.w.K <= QT_MAX_K;
     if constexpr (sizeof(T) == 4) {
         if (a.M <= 4) return launch_tc_q4<T, 4>(a, st);
         if (a.M <= 8) return launch_tc_q4<T, 8>(a, st);
         if (a.M <= 16) return launch_tc_q4<T, 16>(a, st);
         if (a.M <= 32) return launch_tc_q4<T, 32>(a, st);
-        return launch_tc_q4<T, 64>(a, st);
+        return wide ? launch_tc_q4<T, 64, 2>(a, st) : launch_tc_q4<T, 64>(a, st);
     } else {
         if (a.M <= 2) return launch_tc_q4<T, 2>(a, st);
         if (a.M <= 4) return launch_tc_q4<T, 4>(a, st);
         if (a.M <= 8) return launch_tc_q4<T, 8>(a, st);
         if (a.M <= 16) return launch_tc_q4<T, 16>(a, st);
-        return launch_tc_q4<T, 32>(a, st);
+        return wide ? launch_tc_q4<T, 32, 2>(a, st) : launch_tc_q4<T, 32>(a, st);
     }
 }
 template int fc_q4<uint32_t>(const Q4Args<uint32_t> &, cudaStream_t);

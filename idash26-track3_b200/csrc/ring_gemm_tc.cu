@@ -335,9 +335,6 @@ __device__ __forceinline__ void cp_async8(uint32_t dst, const void *src, uint32_
 {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __global__ void __launch_bounds__(TC_THREADS, 1) ring_gemm_tc2_kernel(const __grid_constant__ Gemm2Args a, uint32_t *err)
 {

@@ -62,6 +62,7 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity)
 // after TC_WAIT_NS (or 2^26 polls) without completion
 __device__ inline bool mbar_wait(uint64_t *bar, uint32_t parity)
 {
+    if (mbar_test(bar, parity)) return true;  // the usual case, without reading the timer
     const uint64_t t0 = global_ns();
     for (uint32_t it = 1; it < (1u << 26); ++it) {
         if (mbar_test(bar, parity)) return true;
@@ -69,6 +70,30 @@ __device__ inline bool mbar_wait(uint64_t *bar, uint32_t parity)
     }
     return false;
 }
+
+// one arrival on an mbarrier (release: the caller's earlier writes are visible to who waits)
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// one arrival that also announces `bytes` of asynchronous copies to come
+__device__ __forceinline__ void mbar_expect(uint64_t *bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
+}
+
+// true in one lane of a converged warp.  MMAs issued by an elected lane of a
+// warp-uniform loop keep their descriptors in uniform registers: 4 MMAs and a
+// commit take 500 cycles to issue, against 750 under threadIdx.x == 0.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -124,6 +149,19 @@ __device__ __forceinline__ void store_planes(uint8_t *base, uint32_t plane_bytes
         for (int q = 0; q < 4; q++) *reinterpret_cast<uint32_t *>(base + (4 + q) * plane_bytes + off) = p[q];
     }
 }
+
+// asynchronous copy of `bytes` of N bytes (the rest zeros) to shared memory
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes)
+{
+    if constexpr (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 constexpr int tmem_cols(int n)
 {

@@ -499,8 +499,8 @@ int ddg_op_output_keygen(ddg_dealer *dealer, ddg_cursor *cur, ddg_mask_wire *o);
  * d_q: output n's codes in one row of ddg_q4_row_bytes(K) bytes, code k in the
  * low half (k even) or the high half (k odd) of byte k/2; 16-byte aligned.
  * d_step: ceil(K / group) x N uint16 steps of 12 bits (higher bits are
- * ignored), so that every weight is below 2^15 in magnitude.  group is a
- * multiple of 32.  d_bias2s: N ring elements (bias << scale), or NULL. */
+ * ignored), so that every weight is below 2^15 in magnitude; 4-byte aligned.
+ * group is a multiple of 32.  d_bias2s: N ring elements (bias << scale), or NULL. */
 typedef struct ddg_q4_weights {
     int K, N, group;
     const void *d_q;

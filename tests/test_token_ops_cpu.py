@@ -20,7 +20,7 @@ def la(ddg, batch=1, heads=2, tokens=5, dk=4, dv=3, chunk=4, pow_n=5):
 
 
 @pytest.mark.parametrize("kw", [dict(K=-1), dict(N=-1), dict(group=0), dict(group=48), dict(q=None), dict(step=None),
-                                dict(q=264)])
+                                dict(q=264), dict(step=258)])
 def test_fc_q4_refuses_bad_weights(ddg, kw):
     assert ddg.lib().ddg_fc_q4_share(32, 0, 2, q4(ddg, **kw), 256, 64, 256, 256, None) == ARG
 
