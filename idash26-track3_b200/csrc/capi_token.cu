@@ -31,6 +31,7 @@ int check_linattn(const ddg_linattn_shape *p, LaShape *s)
     s->B = p->batch, s->H = p->heads, s->T = p->tokens, s->dk = p->dk, s->dv = p->dv, s->C = p->chunk;
     s->pn = p->pow_n;
     const double tokens = double(p->tokens < 128 ? 128 : p->tokens);
+    DDG_CHECK(p->tokens <= (1 << 24), DDG_ERR_ARG, "%d tokens in one prompt (at most 2^24)", p->tokens);
     DDG_CHECK(double(p->batch) * p->heads * tokens * 512.0 * 128.0 < 9e18 && double(p->heads) * 384.0 < 2e9,
               DDG_ERR_ARG, "linear attention sizes overflow");
     return DDG_OK;

@@ -9,7 +9,7 @@
 // products with the public decays are local on the masked values.
 //
 // The three matrix stages (scores, chunk states, outputs) run on the tensor
-// cores in la_tile: 128 rows x NT columns of sum_p A_p . B_p, ring operands
+// cores in la_tiles: 128 rows x NT columns of sum_p A_p . B_p, ring operands
 // split into bytes by the loading threads, limb sums
 //   C = sum_s 2^(8s) sum_{i+j=s} A_i . B_j  (u8 x u8 -> s32, exact: K <= 512)
 // in tensor memory.  The limbs of B are stacked along N, so one MMA per limb i
@@ -35,15 +35,15 @@ inline int64_t la_blocks(int64_t n, int V) { return (n + int64_t(LA_THREADS) * V
 #define LA_EACH(e, n) \
     for (int64_t e = int64_t(blockIdx.x) * LA_THREADS + threadIdx.x; e < (n); e += int64_t(gridDim.x) * LA_THREADS)
 
-// chunk and row of entry e of one head's score triangles
+// chunk, row and column of entry e of one head's score triangles (e < 2^31: check_linattn)
 __device__ __forceinline__ void tri_find(const LaShape &s, int64_t e, int &c, int &i, int &j)
 {
-    const int64_t full = int64_t(s.C) * (s.C + 1) / 2;
-    c = int(e / full);
-    const int r = int(e - c * full);
+    const uint32_t full = uint32_t(s.C) * uint32_t(s.C + 1) / 2;
+    c = int(uint32_t(e) / full);
+    const int r = int(uint32_t(e) - uint32_t(c) * full);
     i = int((sqrtf(8.f * float(r) + 1.f) - 1.f) * 0.5f);
-    while ((i + 1) * (i + 2) / 2 <= r) i++;
-    while (i * (i + 1) / 2 > r) i--;
+    if ((i + 1) * (i + 2) / 2 <= r) i++;
+    if (i * (i + 1) / 2 > r) i--;
     j = r - i * (i + 1) / 2;
 }
 
@@ -82,54 +82,61 @@ __global__ void __launch_bounds__(LA_THREADS)
     }
 }
 
-// Scores: V consecutive packed entries per thread, the triangle walked from the
-// first one's position.  States: V columns of up to LC_OT output chunks per
-// thread, every earlier chunk read once per LC_OT outputs; the sums cannot
-// be chained from chunk to chunk, because each S_c is floored from exact terms.
-constexpr int LC_OT = 16;
+// Blocks take a slice of one head's scores or of one head's states.
+// Scores: V packed entries at a time, the triangle walked from the first one's
+// position.  States: V entries of LC_OT output chunks per thread; every earlier
+// chunk is read once per LC_OT outputs, against a table of decays in shared
+// memory.  The sums cannot be chained from chunk to chunk, because each S_c is
+// floored from exact terms.
+constexpr int LC_OT = 16, LC_SLICE = 4096;
 
 template <typename T, int V>
 __global__ void __launch_bounds__(LA_THREADS)
-    k_la_carry(const LaShape s, const T *pow, const T *ps, const T *s0, T *out, int score_blocks)
+    k_la_carry(const LaShape s, const T *pow, const T *ps, const T *s0, T *out, int state_slices, int score_slices,
+               int64_t state_blocks)
 {
-    const int64_t ns = s.n_scores(), tri = s.tri();
-    if (int(blockIdx.x) < score_blocks) {
-        for (int64_t e0 = (int64_t(blockIdx.x) * LA_THREADS + threadIdx.x) * V; e0 < ns;
-             e0 += int64_t(score_blocks) * LA_THREADS * V) {
-            int64_t bh = e0 / tri;
+    __shared__ T w[LC_OT][LC_OT];  // [j][o]: decay from chunk j0 + j to chunk c0 + o
+    const int64_t ns = s.n_scores(), state = s.n_state();
+    const int nc = s.chunks();
+    if (blockIdx.x >= state_blocks) {
+        const uint32_t block = uint32_t(blockIdx.x - state_blocks), bh = block / uint32_t(score_slices);
+        const int64_t tri = s.tri(), base = int64_t(bh) * tri;
+        const T *const pw = pow + int64_t(bh % uint32_t(s.H)) * (s.pn + 1);
+        // whole vectors start on multiples of V of the array, so the head's first may be cut
+        const int64_t lo = (block - bh * uint32_t(score_slices)) * int64_t(LC_SLICE) - base % V;
+        for (int e = threadIdx.x * V; e < LC_SLICE; e += LA_THREADS * V) {
+            const int64_t r0 = lo + e;
+            if (r0 >= tri) break;
+            int skip = r0 < 0 ? int(-r0) : 0, n = tri - r0 < V ? int(tri - r0) : V;
             int c, i, j;
-            tri_find(s, e0 - bh * tri, c, i, j);
-            const int n = ns - e0 < V ? int(ns - e0) : V;
+            tri_find(s, r0 + skip, c, i, j);
+            int len = s.len(c);
             Pack<T, V> v;
-            if (n == V)
-                v = *reinterpret_cast<const Pack<T, V> *>(ps + e0);
+            if (!skip && n == V)
+                v = *reinterpret_cast<const Pack<T, V> *>(ps + base + r0);
             else
-                for (int k = 0; k < n; k++) v.e[k] = ps[e0 + k];
-            const T *pw = pow + bh % s.H * (s.pn + 1);
+                for (int k = skip; k < n; k++) v.e[k] = ps[base + r0 + k];
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                if (k >= n) break;
+                if (k < skip || k >= n) continue;
                 v.e[k] *= __ldg(pw + i - j);
-                if (++j > i) {  // next row, chunk or head
+                if (++j > i) {  // next row or chunk
                     j = 0;
-                    if (++i >= s.len(c)) {
-                        i = 0;
-                        if (++c >= s.chunks()) c = 0, bh++, pw = pow + bh % s.H * (s.pn + 1);
-                    }
+                    if (++i >= len && c + 1 < nc) i = 0, len = s.len(++c);
                 }
             }
-            if (n == V)
-                *reinterpret_cast<Pack<T, V> *>(out + e0) = v;
+            if (!skip && n == V)
+                *reinterpret_cast<Pack<T, V> *>(out + base + r0) = v;
             else
-                for (int k = 0; k < n; k++) out[e0 + k] = v.e[k];
+                for (int k = skip; k < n; k++) out[base + r0 + k] = v.e[k];
         }
         return;
     }
-    const int64_t state = s.n_state(), per = int64_t(s.dk) * s.dv;
-    const int nc = s.chunks();
-    const int64_t r = (int64_t(blockIdx.x - score_blocks) * LA_THREADS + threadIdx.x) * V;
-    if (r >= state) return;
-    const T *const pw = pow + r / per % s.H * (s.pn + 1);
+    const uint32_t block = blockIdx.x, bh = block / uint32_t(state_slices);
+    const int per = s.dk * s.dv, at = int(block - bh * uint32_t(state_slices)) * LA_THREADS * V + threadIdx.x * V;
+    const T *const pw = pow + int64_t(bh % uint32_t(s.H)) * (s.pn + 1);
+    const bool on = at < per;
+    const int64_t r = int64_t(bh) * per + (on ? at : 0);
     const T *const in = ps + ns + r;
     Pack<T, V> first;
 #pragma unroll
@@ -139,99 +146,140 @@ __global__ void __launch_bounds__(LA_THREADS)
         T acc[LC_OT][V];
 #pragma unroll
         for (int o = 0; o < LC_OT; o++) {
-            const T p = c0 + o < nc ? __ldg(pw + s.end(c0 + o)) : T(0);
+            const T p = s0 && c0 + o < nc ? __ldg(pw + s.end(c0 + o)) : T(0);
 #pragma unroll
             for (int k = 0; k < V; k++) acc[o][k] = p * first.e[k];
         }
-        const int jn = c0 + LC_OT < nc ? c0 + LC_OT : nc;
-        for (int j = 0; j < jn; j++) {
-            const Pack<T, V> v = *reinterpret_cast<const Pack<T, V> *>(in + j * state);
-            const int at = s.end(j);
+        for (int j0 = 0; j0 <= c0; j0 += LC_OT) {
+            __syncthreads();
+            {
+                const int j = j0 + threadIdx.x / LC_OT, c = c0 + threadIdx.x % LC_OT;
+                w[threadIdx.x / LC_OT][threadIdx.x % LC_OT] = c < nc && j <= c ? __ldg(pw + s.end(c) - s.end(j)) : T(0);
+            }
+            __syncthreads();
+            const int jn = nc - j0 < LC_OT ? nc - j0 : LC_OT;
+            for (int j = 0; j < jn; j += 4) {
+                Pack<T, V> v[4];
 #pragma unroll
-            for (int o = 0; o < LC_OT; o++) {
-                if (c0 + o >= j && c0 + o < nc) {
-                    const T p = __ldg(pw + s.end(c0 + o) - at);
+                for (int q = 0; q < 4; q++)
+                    v[q] = *reinterpret_cast<const Pack<T, V> *>(in + int64_t(j0 + (j + q < jn ? j + q : j)) * state);
 #pragma unroll
-                    for (int k = 0; k < V; k++) acc[o][k] += p * v.e[k];
-                }
+                for (int q = 0; q < 4; q++)
+#pragma unroll
+                    for (int o = 0; o < LC_OT; o++) {
+                        const T p = j + q < jn ? w[j + q][o] : T(0);
+#pragma unroll
+                        for (int k = 0; k < V; k++) acc[o][k] += p * v[q].e[k];
+                    }
             }
         }
+        if (on)
 #pragma unroll
-        for (int o = 0; o < LC_OT; o++) {
-            if (c0 + o >= nc) break;
-            Pack<T, V> v;
+            for (int o = 0; o < LC_OT; o++) {
+                if (c0 + o >= nc) break;
+                Pack<T, V> v;
 #pragma unroll
-            for (int k = 0; k < V; k++) v.e[k] = acc[o][k];
-            *reinterpret_cast<Pack<T, V> *>(out + ns + (c0 + o) * state + r) = v;
-        }
+                for (int k = 0; k < V; k++) v.e[k] = acc[o][k];
+                *reinterpret_cast<Pack<T, V> *>(out + ns + (c0 + o) * state + r) = v;
+            }
     }
 }
 
 // ------------------------------------------------------------------ matrix stages
 
+// Persistent kernels, two CTAs per SM over strided lists of tiles.  Eight warps
+// load the operands of the next K-step into registers (no detour through shared
+// memory, whose bandwidth the planes and the MMAs' own reads take), split the
+// present one into planes and hand a stage to the MMA warp by mbarrier; there is
+// no CTA-wide barrier in the loop, and loads run on across tiles.  What bounds
+// these kernels is the latency of that chain in each warp (2000 cycles a step
+// with one CTA per SM), then the loads' lines in flight, so there are two CTAs,
+// every load covers whole 128-byte lines, and whole tiles take loads without
+// bounds.
+constexpr int LT_WARPS = 8, LT_THREADS = LT_WARPS * 32;
+
 template <typename T>
 struct LtShape {
     static constexpr int P = int(sizeof(T));
-    static constexpr int NT = 256 / P;             // tile columns: P x NT = 256 accumulator columns, two CTAs an SM
-    static constexpr int NSTAGE = 2;
+    static constexpr int NT = 256 / P;             // tile columns: P x NT = 256 accumulator columns
+    static constexpr int NSTAGE = P == 4 ? 3 : 2;
     // 8-row groups of the operand planes 272 instead of 256 bytes apart: the
     // transposing loaders store rows 4 apart, which then fall on distinct banks
     static constexpr uint32_t SBO = 272;
     static constexpr uint32_t A_PLANE = TC_BM / 8 * SBO, B_PLANE = NT / 8 * SBO;
     static constexpr uint32_t STAGE = P * (A_PLANE + B_PLANE);
-    static constexpr int BI = NT * 8 / LA_THREADS;  // 4-element items of B per thread
-    static constexpr uint32_t SMEM = 64 + 1024 + NSTAGE * STAGE + 4096;
-    static_assert(TC_BM * (NT + 1) * sizeof(T) <= NSTAGE * STAGE, "the output tile is staged in the operand stages");
+    // the output tile on its way to whole-row stores lies in the stages, empty between two tiles
+    static_assert(TC_BM * (NT + 1) * sizeof(T) <= NSTAGE * STAGE, "output tile");
+    static constexpr uint32_t DESC = LT_WARPS * 4 * 192;            // every warp's descriptions of the tiles in hand
+    static constexpr uint32_t SMEM = 128 + 1024 + NSTAGE * STAGE + DESC + 1024;
 };
 
-// n <= 4 elements at p, zeros behind them
+template <typename T>
+__device__ __forceinline__ bool aligned16(const T *p, int64_t ld)
+{
+    return ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld * int64_t(sizeof(T)))) & 15) == 0;
+}
+
+// four elements at p as 16-byte accesses
+template <typename T>
+__device__ __forceinline__ void load4(const T *p, T (&e)[4])
+{
+#pragma unroll
+    for (int i = 0; i < int(sizeof(T)) / 4; i++)
+        *reinterpret_cast<uint4 *>(e + i * (16 / int(sizeof(T)))) = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+}
+// the first n of them, zeros behind; vec: 16-byte accesses where all four are there
 template <typename T>
 __device__ __forceinline__ void load4(const T *p, int n, bool vec, T (&e)[4])
 {
     if (vec && n >= 4) {
-        const uint4 *v = reinterpret_cast<const uint4 *>(p);
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T)) / 4; i++) *reinterpret_cast<uint4 *>(e + i * (16 / int(sizeof(T)))) = __ldg(v + i);
+        load4<T>(p, e);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) e[i] = i < n ? __ldg(p + i) : T(0);
     }
 }
 
+// Which product a tile belongs to, by how its operands lie.
+//   LT_SCORES  A = q (rows of k), B = k (rows of k)
+//   LT_STATES  A = Kd, B = V (both k-major: a row per token)
+//   LT_OUTPUT  first A = P (packed causal triangle), B = V (k-major), then A = Qd (rows of k), B = S (k-major)
+enum { LT_SCORES = 0, LT_STATES = 1, LT_OUTPUT = 2 };
 template <typename T>
-__device__ __forceinline__ bool vec_ok(const T *p, int64_t ld)
-{
-    return ((reinterpret_cast<uintptr_t>(p) | uintptr_t(ld * int64_t(sizeof(T)))) & 15) == 0;
-}
-
-// One K-step's operands.  A: rows of K elements (a_t = 0), K rows of elements
-// (1), or packed triangle rows (2, row i at a + i (i + 1) / 2, entries j <= i).
-// B: N rows of K elements (b_t = 0) or K rows of N elements (1); its value is
-// p0 * b - bm, or -b when neg.
-template <typename T>
-struct LtStep {
-    const T *a, *b, *bm;
+struct LtPair {
+    const T *a, *a_ms, *b, *b_ms;
     int64_t lda, ldb;
-    int k0, K, rows, cols;
-    bool a_vec, b_vec, neg;
+    int K;
+    bool vec_a, vec_b;      // 16-byte boundaries
+    bool whole_a, whole_b;  // and every load inside
 };
 
-enum { LT_SCORES = 0, LT_STATES = 1, LT_OUTPUT = 2 };
+// A tile: rows x cols valid of 128 x NT, column j of row i at at + stride * i + j
+// (scores: at + i (i + 1) / 2 + j, entries with j0 + j <= i)
+template <typename T>
+struct LtTile {
+    LtPair<T> p[2];
+    int steps0, steps;  // K-steps of the first pair, of all
+    int rows, cols, j0;
+    int64_t at, stride;
+};
 
-// rows x cols of one output tile: step(s) gives K-step s of `steps`, at(row)
-// the index of its first column in out and z (columns up to last(row))
-template <typename T, int KIND, class Step, class At, class Last>
-__device__ __forceinline__ void la_tile(int steps, T p0, Step step, int rows, At at, Last last, const T *z, T *out,
-                                        uint32_t *err)
+__device__ __forceinline__ void expander_sync() { asm volatile("bar.sync 1, %0;" ::"n"(LT_THREADS) : "memory"); }
+
+// Tiles first, first + step, .. below `tiles`; tile_of(index) describes one.
+// beaver: with the mask-share products (odd K-steps are -[a] . b), else the
+// plain product (the dealer's word).
+template <typename T, int KIND, class TileOf>
+__device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t tiles, TileOf tile_of, T p0, bool beaver,
+                                         const T *z, T *out, uint32_t *err)
 {
     using S = LtShape<T>;
-    constexpr int P = S::P, NT = S::NT, BI = S::BI;
-    constexpr bool B_T = KIND != LT_SCORES;
+    constexpr int P = S::P, NT = S::NT, NST = S::NSTAGE;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint64_t *const bars = reinterpret_cast<uint64_t *>(smem_raw);
-    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem_raw + 32);
-    uint8_t *const smem = smem_raw + 64 + ((1024u - ((smem_addr(smem_raw) + 64u) & 1023u)) & 1023u);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint64_t *const empty = reinterpret_cast<uint64_t *>(smem_raw), *const full = empty + NST;
+    uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem_raw + 96);
+    uint8_t *const smem = smem_raw + 128 + ((1024u - ((smem_addr(smem_raw) + 128u) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)),
@@ -240,259 +288,361 @@ __device__ __forceinline__ void la_tile(int steps, T p0, Step step, int rows, At
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < S::NSTAGE; i++) mbar_init(bars + i, 1);
+        for (int i = 0; i < NST; i++) mbar_init(empty + i, 1), mbar_init(full + i, LT_WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    // A wait that gave up turns `ok` off: the warp then runs through its remaining
+    // arrivals and barriers without waiting or writing, and the launch reports it.
+    bool ok = true;
 
-    // K-contiguous items: 8 rows x 4 quads of k per warp; transposed 4 x 4
-    // blocks: 8 row quads x 4 quads of k per warp
-    const int kq = 4 * (warp & 1) + (lane & 3), krow = 8 * (warp >> 1) + (lane >> 2);
-    const int tkq = 4 * (warp & 1) + (lane >> 3), trow = 4 * (8 * (warp >> 1) + (lane & 7));
-    T ra[4][4];
-    T rb[B_T ? 4 : BI][4], rm[B_T ? 4 : BI][4];
-    bool neg = false;
-    const bool b_on = !B_T || trow < NT;
-
-    auto load_stage = [&](int s) {
-        const LtStep<T> o = step(s);
-        neg = o.neg;
-        if constexpr (KIND == LT_STATES) {
+    if (warp == LT_WARPS) {
+        const bool leader = elect_one();
+        uint32_t g = 0;  // K-steps so far
+        for (int64_t t = first; t < tiles; t += step) {
+            const int steps = tile_of(t).steps;
+            for (int s = 0; s < steps; s++, g++) {
+                const uint32_t st = g % NST;
+                if (ok) ok = mbar_wait(&full[st], (g / NST) & 1);
+                tc_fence_after();
+                if (ok && leader) {
+                    const uint32_t sa = smem_addr(smem + st * S::STAGE);
+                    const uint64_t db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int k = o.k0 + 4 * tkq + t;
-                load4<T>(o.a + int64_t(k) * o.lda + trow, k < o.K ? o.rows - trow : 0, o.a_vec, ra[t]);
+                    for (int i = 0; i < P; i++)
+                        mma_i8(tmem + uint32_t(i * NT), smem_desc(sa + i * S::A_PLANE, 128, S::SBO), db,
+                               i8_idesc((P - i) * NT, false), (s > 0 || i > 0) ? 1u : 0u);
+                    mma_commit(&empty[st]);
+                }
+                __syncwarp();
             }
-        } else {
+        }
+    } else {
+        // This thread's items of a K-step.  Rows of k: A rows krow + 32 j, B rows (columns of the tile)
+        // brow + 32 j, four k from 4 kq.  k-major: 4 x 4 blocks of rows trow.. and k 4 tkq.. .
+        constexpr bool A_T = KIND == LT_STATES, B_T = KIND != LT_SCORES;
+        // (P = 8: 32 columns; one column and four k a thread, to save registers)
+        constexpr bool B_ONE = B_T && P == 8;
+        constexpr int BI = B_ONE ? 1 : B_T ? 4 : NT / 32;
+        const int kq = 4 * (warp & 1) + (lane & 3), krow = 8 * (warp >> 1) + (lane >> 2);
+        const int tkq = 4 * (warp & 1) + (lane >> 3), trow = 4 * (8 * (warp >> 1) + (lane & 7));
+        const int bcol = 8 * (warp >> 1) + (lane & 7);
+        const bool b_on = !B_T || B_ONE || trow < NT;
+        struct Regs {
+            T a[4][4], b[BI][4], m[BI][4];
+            bool neg;
+        };
+
+        auto load = [&](const LtTile<T> &t, int s, Regs &r) {
+            const bool second = KIND == LT_OUTPUT && s >= t.steps0;
+            const LtPair<T> &p = t.p[second ? 1 : 0];
+            const int i = second ? s - t.steps0 : s;
+            r.neg = beaver && (i & 1);
+            const int k0 = (beaver ? i >> 1 : i) * 32;
+            const bool with_m = beaver && !r.neg;
+            const T *const a = r.neg ? p.a_ms : p.a;
+            const int64_t lda = p.lda, ldb = p.ldb;
+            if constexpr (A_T) {
+                const T *q = a + int64_t(k0 + 4 * tkq) * lda + trow;
+                if (p.whole_a) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int row = krow + 32 * j, k = o.k0 + 4 * kq;
-                if (KIND == LT_OUTPUT && o.lda < 0) {  // packed triangle
-                    load4<T>(o.a + row * (row + 1) / 2 + k, row < o.rows ? row + 1 - k : 0, false, ra[j]);
+                    for (int e = 0; e < 4; e++, q += lda) load4<T>(q, r.a[e]);
                 } else {
-                    load4<T>(o.a + row * o.lda + k, row < o.rows ? o.K - k : 0, o.a_vec, ra[j]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++, q += lda) load4<T>(q, k0 + 4 * tkq + e < p.K ? t.rows - trow : 0, p.vec_a, r.a[e]);
+                }
+            } else if (KIND == LT_OUTPUT && !second) {
+                const int k = k0 + 4 * kq;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int row = krow + 32 * j;
+                    load4<T>(a + row * (row + 1) / 2 + k, row < t.rows ? row + 1 - k : 0, false, r.a[j]);
+                }
+            } else {
+                const T *q = a + krow * lda + k0 + 4 * kq;
+                if (p.whole_a) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++, q += 32 * lda) load4<T>(q, r.a[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++, q += 32 * lda)
+                        load4<T>(q, krow + 32 * j < t.rows ? p.K - k0 - 4 * kq : 0, p.vec_a, r.a[j]);
                 }
             }
-        }
-        const bool with_m = !o.neg && o.bm;
-        if constexpr (B_T) {
-            if (b_on) {
+            if (!b_on) return;
+            if constexpr (B_ONE) {
+                const int64_t o = int64_t(k0 + 4 * tkq) * ldb + bcol;
+                const int n = p.whole_b ? 4 : bcol < t.cols ? p.K - k0 - 4 * tkq : 0;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int k = o.k0 + 4 * tkq + t, n = k < o.K ? o.cols - trow : 0;
-                    const int64_t off = int64_t(k) * o.ldb + trow;
-                    load4<T>(o.b + off, n, o.b_vec, rb[t]);
-                    load4<T>(o.bm + off, with_m ? n : 0, o.b_vec, rm[t]);
+                for (int e = 0; e < 4; e++) {
+                    r.b[0][e] = e < n ? __ldg(p.b + o + e * ldb) : T(0);
+                    if (with_m) r.m[0][e] = e < n ? __ldg(p.b_ms + o + e * ldb) : T(0);
+                }
+                return;
+            }
+            const int64_t o = B_T ? int64_t(k0 + 4 * tkq) * ldb + trow : krow * ldb + k0 + 4 * kq;
+            const int64_t inc = B_T ? ldb : 32 * ldb;
+            const T *q = p.b + o, *m = p.b_ms + o;
+            if (p.whole_b) {
+#pragma unroll
+                for (int e = 0; e < BI; e++, q += inc) load4<T>(q, r.b[e]);
+                if (with_m) {
+#pragma unroll
+                    for (int e = 0; e < BI; e++, m += inc) load4<T>(m, r.m[e]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < BI; e++, q += inc, m += inc) {
+                    const int n = B_T ? (k0 + 4 * tkq + e < p.K ? t.cols - trow : 0)
+                                      : (krow + 32 * e < t.cols ? p.K - k0 - 4 * kq : 0);
+                    load4<T>(q, n, p.vec_b, r.b[e]);
+                    if (with_m) load4<T>(m, n, p.vec_b, r.m[e]);
                 }
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < BI; j++) {
-                const int w = warp + 8 * j, n = 8 * (w >> 1) + (lane >> 2), k = o.k0 + 16 * (w & 1) + 4 * (lane & 3);
-                const int cnt = n < o.cols ? o.K - k : 0;
-                const int64_t off = int64_t(n) * o.ldb + k;
-                load4<T>(o.b + off, cnt, o.b_vec, rb[j]);
-                load4<T>(o.bm + off, with_m ? cnt : 0, o.b_vec, rm[j]);
-            }
-        }
-    };
-    auto store_stage = [&](int st) {
-        uint8_t *const pa = smem + st * S::STAGE, *const pb = pa + P * S::A_PLANE;
+        };
         auto at_off = [](int row, int q) -> uint32_t {
             return (row >> 3) * S::SBO + (q >> 2) * 128 + (row & 7) * 16 + (q & 3) * 4;
         };
+        const uint32_t a_off = A_T ? at_off(trow, tkq) : at_off(krow, kq), a_inc = A_T ? 16 : 4 * S::SBO;
+        const uint32_t b_off = B_ONE ? at_off(bcol, tkq) : B_T ? at_off(trow, tkq) : at_off(krow, kq), b_inc = B_T ? 16 : 4 * S::SBO;
+        auto split = [&](Regs &r, uint32_t st) {
+            uint8_t *const pa = smem + st * S::STAGE + a_off, *const pb = smem + st * S::STAGE + P * S::A_PLANE + b_off;
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if constexpr (KIND == LT_STATES) {
-                const T e[4] = {ra[0][j], ra[1][j], ra[2][j], ra[3][j]};
-                store_planes<T>(pa, S::A_PLANE, at_off(trow + j, tkq), e);
-            } else {
-                store_planes<T>(pa, S::A_PLANE, at_off(krow + 32 * j, kq), ra[j]);
+            for (int j = 0; j < 4; j++) {
+                const T e[4] = {A_T ? r.a[0][j] : r.a[j][0], A_T ? r.a[1][j] : r.a[j][1], A_T ? r.a[2][j] : r.a[j][2],
+                                A_T ? r.a[3][j] : r.a[j][3]};
+                store_planes<T>(pa, S::A_PLANE, j * a_inc, e);
             }
-        }
+            if (!b_on) return;
+            if (r.neg) {
 #pragma unroll
-        for (int i = 0; i < (B_T ? 4 : BI); i++)
+                for (int i = 0; i < BI; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) rb[i][e] = neg ? T(0) - rb[i][e] : p0 * rb[i][e] - rm[i][e];
-        if constexpr (B_T) {
-            if (b_on) {
+                    for (int e = 0; e < 4; e++) r.b[i][e] = T(0) - r.b[i][e];
+            } else if (beaver) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const T e[4] = {rb[0][j], rb[1][j], rb[2][j], rb[3][j]};
-                    store_planes<T>(pb, S::B_PLANE, at_off(trow + j, tkq), e);
-                }
+                for (int i = 0; i < BI; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) r.b[i][e] = p0 * r.b[i][e] - r.m[i][e];
             }
-        } else {
 #pragma unroll
             for (int j = 0; j < BI; j++) {
-                const int w = warp + 8 * j;
-                store_planes<T>(pb, S::B_PLANE, at_off(8 * (w >> 1) + (lane >> 2), 4 * (w & 1) + (lane & 3)), rb[j]);
+                constexpr bool X = B_T && !B_ONE;
+                const T e[4] = {X ? r.b[0][j] : r.b[j][0], X ? r.b[1 % BI][j] : r.b[j][1], X ? r.b[2 % BI][j] : r.b[j][2],
+                                X ? r.b[3 % BI][j] : r.b[j][3]};
+                store_planes<T>(pb, S::B_PLANE, j * b_inc, e);
             }
-        }
-    };
+        };
 
-    bool ok = true;
-    load_stage(0);
-    for (int s = 0; s < steps; s++) {
-        const int st = s & 1;
-        bool mine = true;
-        if (s >= 2) mine = mbar_wait(&bars[st], uint32_t(((s >> 1) - 1) & 1));
-        if (mine) store_stage(st);
-        if (s + 1 < steps) load_stage(s + 1);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        // CTA-uniform: every thread leaves the loop together if any wait gave up
-        if (!__syncthreads_and(mine ? 1 : 0)) {
-            ok = false;
-            break;
-        }
-        if (tid == 0) {
+        T *const tile = reinterpret_cast<T *>(smem);
+        // one tile's accumulators (complete with K-step `last`) to memory; the next tile's MMAs wait for
+        // planes that every warp hands over only after this
+        auto epilogue = [&](const LtTile<T> &t, uint32_t last) {
+            constexpr int RW = TC_BM / LT_WARPS, CW = NT / 32, U = 8;  // rows per warp, pieces per row, rows in flight
+            if (ok) ok = mbar_wait(&empty[last % NST], (last / NST) & 1);
+            ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
-            const uint32_t sa = smem_addr(smem + st * S::STAGE);
-            const uint64_t db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
+            const int q = warp & 3;
+            if (ok) {
+#pragma unroll 2
+                for (int c = (warp >> 2) * (NT / 2); c < (warp >> 2) * (NT / 2) + NT / 2; c += 8) {
+                    uint32_t v[P][8];
 #pragma unroll
-            for (int i = 0; i < P; i++)
-                mma_i8(tmem + uint32_t(i * NT), smem_desc(sa + i * S::A_PLANE, 128, S::SBO), db,
-                       i8_idesc((P - i) * NT, false), (s > 0 || i > 0) ? 1u : 0u);
-            mma_commit(&bars[st]);
-        }
-    }
-    if (ok) ok = mbar_wait(&bars[(steps - 1) & 1], uint32_t(((steps - 1) >> 1) & 1));
-    const int all_ok = __syncthreads_and(ok ? 1 : 0);
-    tc_fence_after();
-
-    // limb sums -> ring elements, row by row through shared memory for whole-row stores
-    T *const tile = reinterpret_cast<T *>(smem);
-    if (all_ok) {
-        const int q = warp & 3, h = warp >> 2;
-#pragma unroll 1
-        for (int c = h * (NT / 2); c < (h + 1) * (NT / 2); c += 8) {
-            T r[8];
+                    for (int s = 0; s < P; s++)
+                        tmem_ld8(tmem + (uint32_t(32 * q) << 16) + uint32_t(s * NT + c), v[s]);
+                    tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 8; e++) r[e] = 0;
+                    for (int e = 0; e < 8; e++) {
+                        T r = 0;
 #pragma unroll
-            for (int s = 0; s < P; s++) {
-                uint32_t v[8];
-                tmem_ld8(tmem + (uint32_t(32 * q) << 16) + uint32_t(s * NT + c), v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int e = 0; e < 8; e++) r[e] += T(v[e]) << (8 * s);
+                        for (int s = 0; s < P; s++) r += T(v[s][e]) << (8 * s);
+                        tile[(32 * q + lane) * (NT + 1) + c + e] = r;
+                    }
+                }
             }
+            tc_fence_before();
+            expander_sync();
+#pragma unroll 1
+            for (int i0 = 0; i0 < RW; i0 += U) {
+                if (!ok || warp + LT_WARPS * i0 >= t.rows) break;
+                T add[U][CW];
+                const T *zr = z + t.at;
+                T *const orow = out + t.at;
+                auto row_at = [&](int row) {
+                    return KIND == LT_SCORES ? int64_t(row * (row + 1) / 2) : t.stride * row;
+                };
+                auto width = [&](int row) { return row >= t.rows ? 0 : KIND == LT_SCORES ? row + 1 - t.j0 : t.cols; };
 #pragma unroll
-            for (int e = 0; e < 8; e++) tile[(32 * q + lane) * (NT + 1) + c + e] = r[e];
+                for (int i = 0; i < U; i++) {
+                    const int row = warp + LT_WARPS * (i0 + i), w = width(row);
+                    const T *const zp = zr + row_at(row) + lane;
+#pragma unroll
+                    for (int c = 0; c < CW; c++) add[i][c] = lane + 32 * c < w ? zp[32 * c] : T(0);
+                }
+#pragma unroll
+                for (int i = 0; i < U; i++) {
+                    const int row = warp + LT_WARPS * (i0 + i), w = width(row);
+                    T *const op = orow + row_at(row) + lane;
+#pragma unroll
+                    for (int c = 0; c < CW; c++)
+                        if (lane + 32 * c < w) op[32 * c] = tile[row * (NT + 1) + lane + 32 * c] + add[i][c];
+                }
+            }
+            expander_sync();  // the stages may be filled again
+        };
+
+        // the K-steps of this CTA's tiles, one list: loads run a step ahead of the splits
+        static_assert(sizeof(LtTile<T>) <= 192, "tile descriptions");
+        uint8_t *const desc = smem + NST * S::STAGE + warp * 4 * 192;
+        auto slot = [&](uint32_t i) -> LtTile<T> & { return *reinterpret_cast<LtTile<T> *>(desc + (i & 3) * 192); };
+        auto describe = [&](uint32_t i, int64_t index) {  // tile i of this CTA, for the lanes of this warp
+            const LtTile<T> t = tile_of(index);
+            __syncwarp();
+            if (lane == 0) slot(i) = t;
+            __syncwarp();
+        };
+        Regs r;
+        int64_t li = first, ci = first;  // tile being loaded, being split
+        int ls = 0, cs = 0;
+        uint32_t g = 0, n = 0, ln = 0;
+        if (first < tiles) describe(0, first);
+        auto load_next = [&]() {
+            if (li >= tiles) return;
+            load(slot(ln), ls, r);
+            if (++ls == slot(ln).steps) {
+                ls = 0, li += step;
+                if (li < tiles) describe(++ln, li);
+            }
+        };
+        load_next();
+        while (ci < tiles) {
+            const uint32_t st = g % NST;
+            if (g >= NST && ok) ok = mbar_wait(&empty[st], (g / NST - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) split(r, st);
+            load_next();
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]);
+            g++;
+            if (++cs == slot(n).steps) {
+                epilogue(slot(n), g - 1);
+                n++, cs = 0, ci += step;
+            }
         }
-    } else if (tid == 0) {
-        atomicOr(err, 8u);
+        if (!ok && lane == 0) atomicOr(err, 8u);
     }
     tc_fence_before();
     __syncthreads();
-    if (all_ok) {
-        for (int row = warp; row < rows; row += LA_THREADS / 32) {
-            const int64_t o = at(row);
-            const int n = last(row);
-#pragma unroll
-            for (int c = lane; c < NT; c += 32)
-                if (c < n) out[o + c] = tile[row * (NT + 1) + c] + z[o + c];
-        }
-    }
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
     }
 }
 
-// tiles of chunk c of head bh: score columns 0, NT, .. then state columns 0, NT, ..
+inline __host__ __device__ int steps32(int k) { return (k + 31) / 32; }
+
+// CTAs below score_ctas take score tiles (columns 0, NT, .. of each chunk), the others state tiles
 template <typename T>
-__global__ void __launch_bounds__(LA_THREADS, 2)
-    k_la_chunk(const LaShape s, const __grid_constant__ LaChunkArgs<T> a, int score_tiles, int state_tiles, uint32_t *err)
+__global__ void __launch_bounds__(LT_THREADS + 32, 2)
+    k_la_chunk(const LaShape s, const __grid_constant__ LaChunkArgs<T> a, int score_tiles, int state_tiles, int score_ctas,
+               uint32_t *err)
 {
     constexpr int NT = LtShape<T>::NT;
-    const int per = score_tiles + state_tiles, which = blockIdx.x % per;
-    const int64_t bc = blockIdx.x / per, bh = bc / s.chunks();
-    const int c = int(bc - bh * s.chunks()), len = s.len(c);
-    const int64_t b = bh / s.H, h = bh - b * s.H;
-    const int64_t row0 = (b * s.T + int64_t(c) * s.C) * a.ld;
-    if (which < score_tiles) {
-        const int j0 = which * NT;
-        if (j0 >= len) return;
-        const int64_t oq = row0 + h * s.dk, ok = oq + int64_t(s.H) * s.dk;
-        const bool qv = vec_ok(a.qkv + oq, a.ld) && vec_ok(a.qkv_ms + oq, a.ld);
-        const bool kv = vec_ok(a.qkv + ok, a.ld) && vec_ok(a.qkv_ms + ok, a.ld);
-        const int nd = (s.dk + 31) / 32;
-        const int64_t o = bh * s.tri() + s.tri_at(c) + j0;
-        la_tile<T, LT_SCORES>(
-            a.qkv_ms ? 2 * nd : nd, a.p0,
-            [&](int i) {
-                const bool neg = a.qkv_ms && (i & 1);
-                LtStep<T> r;
-                r.a = (neg ? a.qkv_ms : a.qkv) + oq, r.lda = a.ld, r.a_vec = qv, r.rows = len;
-                r.b = a.qkv + ok + j0 * a.ld, r.bm = a.qkv_ms ? a.qkv_ms + ok + j0 * a.ld : nullptr;
-                r.ldb = a.ld, r.b_vec = kv, r.cols = len - j0;
-                r.k0 = (a.qkv_ms ? i >> 1 : i) * 32, r.K = s.dk, r.neg = neg;
-                return r;
-            },
-            len, [&](int i) { return o + int64_t(i) * (i + 1) / 2; }, [&](int i) { return i + 1 - j0; }, a.z, a.out, err);
+    const int two = a.qkv_ms ? 2 : 1, nc = s.chunks();
+    const int64_t chunks = s.bh() * nc, kd0 = int64_t(s.H) * s.dk;
+    struct Spot {
+        int64_t b, h, bh, row0;
+        int c, len, which;
+    };
+    auto find = [&](int64_t index, int per) {
+        Spot f;
+        // heads before chunks before sequences: what runs at one time reads whole q|k|v rows
+        const int64_t r = index / per, bc = r / s.H;
+        f.which = int(index - r * per), f.h = r - bc * s.H, f.b = bc / nc, f.c = int(bc - f.b * nc);
+        f.bh = f.b * s.H + f.h, f.len = s.len(f.c);
+        f.row0 = (f.b * s.T + int64_t(f.c) * s.C) * a.ld;
+        return f;
+    };
+    if (int(blockIdx.x) < score_ctas) {
+        auto tile_of = [&](int64_t index) {
+            const Spot f = find(index, score_tiles);
+            const int j0 = f.which * NT;
+            const int64_t oq = f.row0 + f.h * s.dk, ok = oq + kd0 + int64_t(j0) * a.ld;
+            LtTile<T> t;
+            LtPair<T> &p = t.p[0];
+            p.a = a.qkv + oq, p.a_ms = a.qkv_ms + oq, p.b = a.qkv + ok, p.b_ms = a.qkv_ms + ok;
+            p.lda = p.ldb = a.ld, p.K = s.dk;
+            // a short chunk's last column tiles may be empty: no rows
+            t.rows = j0 < f.len ? f.len : 0, t.cols = j0 < f.len ? f.len - j0 : 0, t.j0 = j0;
+            p.vec_a = aligned16(p.a, a.ld) && aligned16(p.a_ms, a.ld);
+            p.vec_b = aligned16(p.b, a.ld) && aligned16(p.b_ms, a.ld);
+            p.whole_a = p.vec_a && t.rows == TC_BM && s.dk % 32 == 0;
+            p.whole_b = p.vec_b && t.cols >= NT && s.dk % 32 == 0;
+            t.at = f.bh * s.tri() + s.tri_at(f.c) + j0, t.stride = 0;
+            t.steps0 = t.steps = two * steps32(s.dk);
+            return t;
+        };
+        la_tiles<T, LT_SCORES>(blockIdx.x, score_ctas, chunks * score_tiles, tile_of, a.p0, two == 2, a.z, a.out, err);
     } else {
-        const int y0 = (which - score_tiles) * NT;
-        const int64_t ok = (bh * s.T + int64_t(c) * s.C) * s.dk;
-        const int64_t ov = row0 + 2 * int64_t(s.H) * s.dk + h * s.dv + y0;
-        const bool kv = vec_ok(a.kd + ok, s.dk) && vec_ok(a.kd_ms + ok, s.dk);
-        const bool vv = vec_ok(a.qkv + ov, a.ld) && vec_ok(a.qkv_ms + ov, a.ld);
-        const int nl = (len + 31) / 32;
-        const int64_t o = s.n_scores() + ((int64_t(c) * s.bh() + bh) * s.dk) * s.dv + y0;
-        la_tile<T, LT_STATES>(
-            a.qkv_ms ? 2 * nl : nl, a.p0,
-            [&](int i) {
-                const bool neg = a.qkv_ms && (i & 1);
-                LtStep<T> r;
-                r.a = (neg ? a.kd_ms : a.kd) + ok, r.lda = s.dk, r.a_vec = kv, r.rows = s.dk;
-                r.b = a.qkv + ov, r.bm = a.qkv_ms ? a.qkv_ms + ov : nullptr, r.ldb = a.ld, r.b_vec = vv;
-                r.cols = s.dv - y0, r.k0 = (a.qkv_ms ? i >> 1 : i) * 32, r.K = len, r.neg = neg;
-                return r;
-            },
-            s.dk, [&](int x) { return o + int64_t(x) * s.dv; }, [&](int) { return s.dv - y0; }, a.z, a.out, err);
+        auto tile_of = [&](int64_t index) {
+            const Spot f = find(index, state_tiles);
+            const int y0 = f.which * NT;
+            const int64_t ok = (f.bh * s.T + int64_t(f.c) * s.C) * s.dk, ov = f.row0 + 2 * kd0 + f.h * s.dv + y0;
+            LtTile<T> t;
+            LtPair<T> &p = t.p[0];
+            p.a = a.kd + ok, p.a_ms = a.kd_ms + ok, p.b = a.qkv + ov, p.b_ms = a.qkv_ms + ov;
+            p.lda = s.dk, p.ldb = a.ld, p.K = f.len;
+            t.rows = s.dk, t.cols = s.dv - y0, t.j0 = 0;
+            p.vec_a = aligned16(p.a, s.dk) && aligned16(p.a_ms, s.dk);
+            p.vec_b = aligned16(p.b, a.ld) && aligned16(p.b_ms, a.ld);
+            p.whole_a = p.vec_a && s.dk == TC_BM && f.len % 32 == 0;
+            p.whole_b = p.vec_b && t.cols >= NT && f.len % 32 == 0;
+            t.at = s.n_scores() + (int64_t(f.c) * s.bh() + f.bh) * s.dk * s.dv + y0, t.stride = s.dv;
+            t.steps0 = t.steps = two * steps32(f.len);
+            return t;
+        };
+        la_tiles<T, LT_STATES>(blockIdx.x - score_ctas, gridDim.x - score_ctas, chunks * state_tiles, tile_of, a.p0,
+                               two == 2, a.z, a.out, err);
     }
 }
 
+// tiles of chunk c of head bh: output columns 0, NT, ..
 template <typename T>
-__global__ void __launch_bounds__(LA_THREADS, 2)
-    k_la_output(const LaShape s, const __grid_constant__ LaOutArgs<T> a, int tiles, uint32_t *err)
+__global__ void __launch_bounds__(LT_THREADS + 32, 2)
+    k_la_output(const LaShape s, const __grid_constant__ LaOutArgs<T> a, int64_t count, int tiles, uint32_t *err)
 {
     constexpr int NT = LtShape<T>::NT;
-    const int y0 = int(blockIdx.x % tiles) * NT;
-    const int64_t bc = blockIdx.x / tiles, bh = bc / s.chunks();
-    const int c = int(bc - bh * s.chunks()), len = s.len(c);
-    const int64_t b = bh / s.H, h = bh - b * s.H;
-    const int64_t op = bh * s.tri() + s.tri_at(c), oq = (bh * s.T + int64_t(c) * s.C) * s.dk;
-    const int64_t ov = (b * s.T + int64_t(c) * s.C) * a.ld + 2 * int64_t(s.H) * s.dk + h * s.dv + y0;
-    const int64_t os = (c ? s.n_scores() + int64_t(c - 1) * s.n_state() : 0) + bh * s.dk * s.dv + y0;
-    const T *const st = c ? a.ps : a.s0, *const st_ms = c ? a.ps_ms : a.s0_ms;
-    const bool qv = vec_ok(a.qd + oq, s.dk) && vec_ok(a.qd_ms + oq, s.dk);
-    const bool vv = vec_ok(a.qkv + ov, a.ld) && vec_ok(a.qkv_ms + ov, a.ld);
-    const bool sv = vec_ok(st + os, s.dv) && vec_ok(st_ms + os, s.dv);
-    const int two = a.qkv_ms ? 2 : 1;
-    const int nl = two * ((len + 31) / 32), nd = st ? two * ((s.dk + 31) / 32) : 0;
-    const int64_t o = ((b * s.T + int64_t(c) * s.C) * s.H + h) * s.dv + y0;
-    la_tile<T, LT_OUTPUT>(
-        nl + nd, a.p0,
-        [&](int i) {
-            LtStep<T> r;
-            const bool tri = i < nl;
-            if (!tri) i -= nl;
-            r.neg = two == 2 && (i & 1);
-            r.k0 = i / two * 32, r.cols = s.dv - y0, r.rows = len;
-            if (tri) {
-                r.a = (r.neg ? a.ps_ms : a.ps) + op, r.lda = -1, r.a_vec = false, r.K = len;
-                r.b = a.qkv + ov, r.bm = a.qkv_ms ? a.qkv_ms + ov : nullptr, r.ldb = a.ld, r.b_vec = vv;
-            } else {
-                r.a = (r.neg ? a.qd_ms : a.qd) + oq, r.lda = s.dk, r.a_vec = qv, r.K = s.dk;
-                r.b = st + os, r.bm = a.qkv_ms ? st_ms + os : nullptr, r.ldb = s.dv, r.b_vec = sv;
-            }
-            return r;
-        },
-        len, [&](int i) { return o + int64_t(i) * s.H * s.dv; }, [&](int) { return s.dv - y0; }, a.z, a.out, err);
+    const int two = a.qkv_ms ? 2 : 1, nc = s.chunks();
+    auto tile_of = [&](int64_t index) {
+        const int64_t r = index / tiles, bc = r / s.H, h = r - bc * s.H, b = bc / nc, bh = b * s.H + h;
+        const int y0 = int(index - r * tiles) * NT, c = int(bc - b * nc), len = s.len(c);
+        const int64_t t0 = b * s.T + int64_t(c) * s.C;
+        const int64_t op = bh * s.tri() + s.tri_at(c), oq = (bh * s.T + int64_t(c) * s.C) * s.dk;
+        const int64_t ov = t0 * a.ld + 2 * int64_t(s.H) * s.dk + h * s.dv + y0;
+        const int64_t os = (c ? s.n_scores() + int64_t(c - 1) * s.n_state() : 0) + bh * s.dk * s.dv + y0;
+        const T *const st = c ? a.ps : a.s0, *const st_ms = c ? a.ps_ms : a.s0_ms;
+        LtTile<T> t;
+        LtPair<T> &p = t.p[0], &q = t.p[1];
+        t.rows = len, t.cols = s.dv - y0, t.j0 = 0;
+        p.a = a.ps + op, p.a_ms = a.ps_ms + op, p.b = a.qkv + ov, p.b_ms = a.qkv_ms + ov;
+        p.lda = 0, p.ldb = a.ld, p.K = len, p.vec_a = p.whole_a = false;
+        p.vec_b = aligned16(p.b, a.ld) && aligned16(p.b_ms, a.ld);
+        p.whole_b = p.vec_b && t.cols >= NT && len % 32 == 0;
+        q.a = a.qd + oq, q.a_ms = a.qd_ms + oq, q.b = st + os, q.b_ms = st_ms + os;
+        q.lda = s.dk, q.ldb = s.dv, q.K = s.dk;
+        q.vec_a = aligned16(q.a, s.dk) && aligned16(q.a_ms, s.dk);
+        q.vec_b = aligned16(q.b, s.dv) && aligned16(q.b_ms, s.dv);
+        q.whole_a = q.vec_a && len == TC_BM && s.dk % 32 == 0;
+        q.whole_b = q.vec_b && t.cols >= NT && s.dk % 32 == 0;
+        t.steps0 = two * steps32(len), t.steps = t.steps0 + (st ? two * steps32(s.dk) : 0);
+        t.at = (t0 * s.H + h) * s.dv + y0, t.stride = int64_t(s.H) * s.dv;
+        return t;
+    };
+    la_tiles<T, LT_OUTPUT>(blockIdx.x, gridDim.x, count, tile_of, a.p0, two == 2, a.z, a.out, err);
 }
 
 // ------------------------------------------------------------------ one token
@@ -612,10 +762,8 @@ int la_decay(const LaShape &s, int64_t ld, const T *pow, const T *x, T *out, cud
 }
 
 template <typename K>
-static int la_tile_launch(K kern, uint32_t smem, int64_t blocks, int (&configured)[64], uint32_t **err)
+static int la_tile_ready(K kern, uint32_t smem, int (&configured)[64], uint32_t **err)
 {
-    DDG_CHECK(blocks <= 0x7fffffff, DDG_ERR_ARG, "linear attention: %lld tiles are too many for one call",
-              (long long)blocks);
     int dev = 0;
     DDG_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -625,6 +773,8 @@ static int la_tile_launch(K kern, uint32_t smem, int64_t blocks, int (&configure
     return ring_gemm_err_word(err);
 }
 
+inline unsigned la_tile_grid(int64_t tiles) { return unsigned(tiles < 2 * 148 ? tiles : 2 * 148); }
+
 template <typename T>
 int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
 {
@@ -632,21 +782,28 @@ int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
     using S = LtShape<T>;
     static thread_local int configured[64];
     const int np = (s.len(0) + S::NT - 1) / S::NT, ns = (s.dv + S::NT - 1) / S::NT;
-    const int64_t blocks = s.bh() * s.chunks() * (np + ns);
     uint32_t *err = nullptr;
-    DDG_TRY(la_tile_launch(k_la_chunk<T>, S::SMEM, blocks, configured, &err));
-    k_la_chunk<T><<<unsigned(blocks), LA_THREADS, S::SMEM, st>>>(s, a, np, ns, err);
+    DDG_TRY(la_tile_ready(k_la_chunk<T>, S::SMEM, configured, &err));
+    // two CTAs per SM, shared out by the two lists' K-steps (a tile's epilogue takes about as long as three)
+    const int64_t chunks = s.bh() * s.chunks(), scores = chunks * np, states = chunks * ns;
+    const int64_t grid = scores + states < 2 * 148 ? scores + states : 2 * 148;
+    const double cs = double(scores) * (2 * steps32(s.dk) + 3), ct = double(states) * (2 * steps32(s.len(0)) + 3);
+    int64_t mine = int64_t(double(grid) * cs / (cs + ct) + 0.5);
+    mine = mine < 1 ? 1 : mine > grid - 1 ? grid - 1 : mine;
+    k_la_chunk<T><<<unsigned(grid), LT_THREADS + 32, S::SMEM, st>>>(s, a, np, ns, int(mine), err);
     return launched();
 }
 
 template <typename T, int V>
 static int launch_carry(const LaShape &s, const T *pow, const T *ps, const T *s0, T *out, cudaStream_t st)
 {
-    const int64_t sb = la_blocks(s.n_scores(), V), nb = la_blocks(s.n_state(), V);
-    const int score_blocks = int(sb < 148 * 16 ? sb : 148 * 16);
-    DDG_CHECK(nb + score_blocks <= 0x7fffffff, DDG_ERR_ARG, "linear attention: %lld state entries are too many",
-              (long long)s.n_state());
-    k_la_carry<T, V><<<unsigned(score_blocks + nb), LA_THREADS, 0, st>>>(s, pow, ps, s0, out, score_blocks);
+    const int64_t per = int64_t(s.dk) * s.dv, state_slices = la_blocks(per, V);
+    const int64_t score_slices = (s.tri() + V + LC_SLICE - 1) / LC_SLICE;
+    DDG_CHECK(s.bh() * (state_slices + score_slices) <= 0x7fffffff, DDG_ERR_ARG,
+              "linear attention: %lld score entries are too many for one call", (long long)s.n_scores());
+    // the states first: theirs are the long dependent sums
+    k_la_carry<T, V><<<unsigned(s.bh() * (state_slices + score_slices)), LA_THREADS, 0, st>>>(
+        s, pow, ps, s0, out, int(state_slices), int(score_slices), s.bh() * state_slices);
     return launched();
 }
 
@@ -668,10 +825,10 @@ int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
     using S = LtShape<T>;
     static thread_local int configured[64];
     const int tiles = (s.dv + S::NT - 1) / S::NT;
-    const int64_t blocks = s.bh() * s.chunks() * tiles;
+    const int64_t count = s.bh() * s.chunks() * tiles;
     uint32_t *err = nullptr;
-    DDG_TRY(la_tile_launch(k_la_output<T>, S::SMEM, blocks, configured, &err));
-    k_la_output<T><<<unsigned(blocks), LA_THREADS, S::SMEM, st>>>(s, a, tiles, err);
+    DDG_TRY(la_tile_ready(k_la_output<T>, S::SMEM, configured, &err));
+    k_la_output<T><<<la_tile_grid(count), LT_THREADS + 32, S::SMEM, st>>>(s, a, count, tiles, err);
     return launched();
 }
 

@@ -522,8 +522,8 @@ int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const voi
 
 /* Linear attention  S_t = lambda_h S_{t-1} + k_t v_t^T,  o_t = q_t S_t  (S is
  * dk x dv per head), for prompts in chunks of `chunk` tokens and for one token.
- * batch >= 0, heads >= 1, tokens >= 0, dk, dv and chunk in 1..128; pow_n >=
- * tokens and >= 1.  Arrays, row-major, T = tokens, bh = batch * heads + head:
+ * batch >= 0, heads >= 1, tokens in 0..2^24, dk, dv and chunk in 1..128;
+ * pow_n >= tokens and >= 1.  Arrays, row-major, T = tokens, bh = batch * heads + head:
  *   qkv     (batch, T) rows, ld elements apart, each [q: heads x dk |
  *           k: heads x dk | v: heads x dv], ld >= heads * (2 dk + dv)
  *   pow     (heads, pow_n + 1): lambda_h^n at the scale (ddg_decay_table)

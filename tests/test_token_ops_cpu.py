@@ -45,7 +45,7 @@ def test_fc_q4_null_weights_and_empty_calls(ddg):
 
 @pytest.mark.parametrize("kw", [dict(batch=-1), dict(heads=0), dict(tokens=-1), dict(dk=0), dict(dk=129), dict(dv=0),
                                 dict(dv=129), dict(chunk=0), dict(chunk=129), dict(pow_n=4),
-                                dict(tokens=0, pow_n=0), dict(batch=1 << 30, heads=1 << 20, tokens=1 << 30,
+                                dict(tokens=0, pow_n=0), dict(tokens=(1 << 24) + 1, pow_n=1 << 25), dict(batch=1 << 30, heads=1 << 20, tokens=1 << 30,
                                                               pow_n=1 << 30)])
 def test_linattn_refuses_bad_shapes(ddg, kw):
     L, s = ddg.lib(), la(ddg, **kw)
