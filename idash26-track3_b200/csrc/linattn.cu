@@ -88,10 +88,10 @@ __global__ void __launch_bounds__(LA_THREADS)
 // chunk is read once per LC_OT outputs, against a table of decays in shared
 // memory.  The sums cannot be chained from chunk to chunk, because each S_c is
 // floored from exact terms.
-constexpr int LC_OT = 16, LC_SLICE = 4096;
+constexpr int LC_OT = 8, LC_SLICE = 4 * LA_THREADS;  // slice: vectors per thread
 
 template <typename T, int V>
-__global__ void __launch_bounds__(LA_THREADS)
+__global__ void __launch_bounds__(LA_THREADS, 3)
     k_la_carry(const LaShape s, const T *pow, const T *ps, const T *s0, T *out, int state_slices, int score_slices,
                int64_t state_blocks)
 {
@@ -103,32 +103,43 @@ __global__ void __launch_bounds__(LA_THREADS)
         const int64_t tri = s.tri(), base = int64_t(bh) * tri;
         const T *const pw = pow + int64_t(bh % uint32_t(s.H)) * (s.pn + 1);
         // whole vectors start on multiples of V of the array, so the head's first may be cut
-        const int64_t lo = (block - bh * uint32_t(score_slices)) * int64_t(LC_SLICE) - base % V;
-        for (int e = threadIdx.x * V; e < LC_SLICE; e += LA_THREADS * V) {
-            const int64_t r0 = lo + e;
+        const int64_t lo = (block - bh * uint32_t(score_slices)) * int64_t(LC_SLICE * V) - base % V;
+        constexpr int PER = LC_SLICE / LA_THREADS;
+        Pack<T, V> v[PER];
+        // every load before the first use: what is in flight is what this part's time goes by
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const int64_t r0 = lo + (p * LA_THREADS + int(threadIdx.x)) * V;
+            if (r0 >= 0 && r0 + V <= tri)
+                v[p] = *reinterpret_cast<const Pack<T, V> *>(ps + base + r0);
+            else
+#pragma unroll
+                for (int k = 0; k < V; k++) v[p].e[k] = r0 + k >= 0 && r0 + k < tri ? ps[base + r0 + k] : T(0);
+        }
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+            const int64_t r0 = lo + (p * LA_THREADS + int(threadIdx.x)) * V;
             if (r0 >= tri) break;
-            int skip = r0 < 0 ? int(-r0) : 0, n = tri - r0 < V ? int(tri - r0) : V;
+            const int skip = r0 < 0 ? int(-r0) : 0, n = tri - r0 < V ? int(tri - r0) : V;
+            if (skip >= n) continue;
             int c, i, j;
             tri_find(s, r0 + skip, c, i, j);
             int len = s.len(c);
-            Pack<T, V> v;
-            if (!skip && n == V)
-                v = *reinterpret_cast<const Pack<T, V> *>(ps + base + r0);
-            else
-                for (int k = skip; k < n; k++) v.e[k] = ps[base + r0 + k];
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 if (k < skip || k >= n) continue;
-                v.e[k] *= __ldg(pw + i - j);
+                v[p].e[k] *= __ldg(pw + i - j);
                 if (++j > i) {  // next row or chunk
                     j = 0;
                     if (++i >= len && c + 1 < nc) i = 0, len = s.len(++c);
                 }
             }
             if (!skip && n == V)
-                *reinterpret_cast<Pack<T, V> *>(out + base + r0) = v;
+                *reinterpret_cast<Pack<T, V> *>(out + base + r0) = v[p];
             else
-                for (int k = skip; k < n; k++) out[base + r0 + k] = v.e[k];
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    if (k >= skip && k < n) out[base + r0 + k] = v[p].e[k];
         }
         return;
     }
@@ -152,7 +163,7 @@ __global__ void __launch_bounds__(LA_THREADS)
         }
         for (int j0 = 0; j0 <= c0; j0 += LC_OT) {
             __syncthreads();
-            {
+            if (threadIdx.x < LC_OT * LC_OT) {
                 const int j = j0 + threadIdx.x / LC_OT, c = c0 + threadIdx.x % LC_OT;
                 w[threadIdx.x / LC_OT][threadIdx.x % LC_OT] = c < nc && j <= c ? __ldg(pw + s.end(c) - s.end(j)) : T(0);
             }
@@ -653,7 +664,7 @@ __global__ void __launch_bounds__(LT_THREADS + 32, 2)
 // bound by memory); q . S comes out of the same pass, summed over the thread
 // rows in shared memory.
 template <typename T, int V>
-__global__ void __launch_bounds__(LA_THREADS)
+__global__ void __launch_bounds__(LA_THREADS, 3)
     k_la_step(const LaShape s, const __grid_constant__ LaStepArgs<T> a, int cx, int slabs)
 {
     __shared__ T qs[128], ks[128], rq[128], rk[128];
@@ -666,6 +677,22 @@ __global__ void __launch_bounds__(LA_THREADS)
     const int64_t oq = b * a.ld + int64_t(h) * s.dk, ok = oq + int64_t(s.H) * s.dk;
     const int64_t ov = b * a.ld + 2 * int64_t(s.H) * s.dk + int64_t(h) * s.dv + col;
     const bool on = col < s.dv;
+    // a thread's next U rows, in flight while the present ones are worked on (the
+    // first ones while q, k and v arrive)
+    constexpr int U = 4;
+    PV S[U], m[U], z[U];
+    const int64_t at = bh * per + col;
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * ry;
+            if (!on || i >= s.dk) continue;
+            const int64_t o = at + int64_t(i) * s.dv;
+            S[u] = *reinterpret_cast<const PV *>(a.s + o), z[u] = *reinterpret_cast<const PV *>(a.z + o);
+            if (a.qkv_ms) m[u] = *reinterpret_cast<const PV *>(a.s_ms + o);
+        }
+    };
+    fetch(y0);
     T v[V], vr[V], acc[V];
 #pragma unroll
     for (int k = 0; k < V; k++) {
@@ -679,26 +706,21 @@ __global__ void __launch_bounds__(LA_THREADS)
     }
     const T lam = a.lam * __ldg(a.pow + int64_t(h) * (s.pn + 1) + 1);
     __syncthreads();
-    if (on) {
-        const int64_t at = bh * per + col;
-#pragma unroll 4
-        for (int i = y0; i < s.dk; i += ry) {
-            const int64_t o = at + int64_t(i) * s.dv;
-            const PV S = *reinterpret_cast<const PV *>(a.s + o), z = *reinterpret_cast<const PV *>(a.z + o);
-            PV m, u;
-            if (a.qkv_ms)
-                m = *reinterpret_cast<const PV *>(a.s_ms + o);
-            else
+    for (int i0 = y0; i0 < s.dk; i0 += U * ry) {
 #pragma unroll
-                for (int k = 0; k < V; k++) m.e[k] = 0;
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * ry;
+            if (!on || i >= s.dk) continue;
             const T q = qs[i], key = ks[i], mq = rq[i], mk = rk[i];
+            PV n;
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                u.e[k] = z.e[k] + lam * S.e[k] + key * vr[k] - mk * v[k];
-                acc[k] += q * (a.p0 * S.e[k] - m.e[k]) - mq * S.e[k];
+                n.e[k] = z[u].e[k] + lam * S[u].e[k] + key * vr[k] - mk * v[k];
+                acc[k] += q * (a.p0 * S[u].e[k] - (a.qkv_ms ? m[u].e[k] : T(0))) - mq * S[u].e[k];
             }
-            *reinterpret_cast<PV *>(a.out + o) = u;
+            *reinterpret_cast<PV *>(a.out + at + int64_t(i) * s.dv) = n;
         }
+        fetch(i0 + U * ry);
     }
 #pragma unroll
     for (int k = 0; k < V; k++) red[tid].e[k] = acc[k];
@@ -798,7 +820,7 @@ template <typename T, int V>
 static int launch_carry(const LaShape &s, const T *pow, const T *ps, const T *s0, T *out, cudaStream_t st)
 {
     const int64_t per = int64_t(s.dk) * s.dv, state_slices = la_blocks(per, V);
-    const int64_t score_slices = (s.tri() + V + LC_SLICE - 1) / LC_SLICE;
+    const int64_t score_slices = (s.tri() + V + LC_SLICE * V - 1) / (LC_SLICE * V);
     DDG_CHECK(s.bh() * (state_slices + score_slices) <= 0x7fffffff, DDG_ERR_ARG,
               "linear attention: %lld score entries are too many for one call", (long long)s.n_scores());
     // the states first: theirs are the long dependent sums
