@@ -228,30 +228,32 @@ constexpr uint32_t QT_A_CHUNK = TC_BM * 16;
 template <typename T, int MT, int NA>
 struct QtShape {
     static constexpr int P = int(sizeof(T));
-    static constexpr int THREADS = NA * Q4_THREADS;                // splitting threads, before the MMA warp
     static constexpr int NB = P * MT;                              // MMA columns
-    // k per stage: narrow MMAs are issue-bound (a commit takes as long as five
-    // of them), so they get twice the K per commit and the SM to themselves
-    static constexpr int KC = NB <= 64 ? 128 : 64, UPT = KC / 64, CTAS = NB == 128 ? 2 : 1;
+    // k per stage: narrower MMAs are issue-bound (a commit takes as long as five
+    // of them), so they get twice the K per commit
+    static constexpr int KC = NB <= 128 ? 128 : 64;
+    static constexpr int BOXES = KC / 64;                          // 32-byte boxes of codes per row and stage
+    // sixteen warps to expand; a unit of codes for each thread of the first UNITS
+    static constexpr int THREADS = 512, UNITS = NA * BOXES * 256;
     static constexpr int CH = KC / 8, XROW = KC / 8;               // chunks per stage; x items of 8 k per row
     static constexpr int COLS = tmem_cols(NA * NB);
     static constexpr uint32_t B_CHUNK = NB * 16 + 16;
     static constexpr uint32_t A_TILE = CH * QT_A_CHUNK, A_STAGE = NA * A_TILE, STAGE = A_STAGE + CH * B_CHUNK;
     static constexpr int ITEMS = MT * XROW, XPT = (ITEMS + THREADS - 1) / THREADS;
-    // A stage's codes (UPT boxes of 32 bytes a row), x and steps as they lie in
+    // A stage's codes (BOXES of 32 bytes a row), x and steps as they lie in
     // memory, loaded RD stages ahead: the memory needs about 40 KB of codes in
     // flight per SM for its latency.  (Asynchronous 16-byte copies by the
     // expanding threads took 600-1000 cycles a stage to issue.)
-    static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = UPT * RAW_BOX, RAW_STEPS = RAW_X + MT * KC * P;
-    static constexpr uint32_t RAW = RAW_STEPS + THREADS * UPT * 4;
-    static constexpr int RD_FIT = int(((CTAS == 2 ? 106 : 212) * 1024 - QT_STAGES * STAGE) / RAW);
+    static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = BOXES * RAW_BOX, RAW_STEPS = RAW_X + MT * KC * P;
+    static constexpr uint32_t RAW = RAW_STEPS + UNITS * 4;
+    static constexpr int RD_FIT = int((212 * 1024 - QT_STAGES * STAGE) / RAW);
     static constexpr int RD = RD_FIT < 2 ? 2 : RD_FIT > 8 ? 8 : RD_FIT;
     // [barriers, TMEM address | sums of x | pad to 1024 | stages | raw stages | slack]
     static constexpr uint32_t HEAD = 256 + MT * P;
     static constexpr uint32_t XPITCH = (ITEMS < THREADS ? ITEMS : THREADS) * 16;  // between 16-byte pieces of the x items
     static constexpr uint32_t SMEM = HEAD + 1024 + QT_STAGES * STAGE + RD * RAW + 2048;
     static_assert(NB % 16 == 0 && NB <= 256 && STAGE % 128 == 0 && RAW % 128 == 0 && RAW_X % 128 == 0, "tile");
-    static_assert(THREADS % XROW == 0 && (ITEMS % THREADS == 0 || XPT == 1), "x items");
+    static_assert(UNITS <= THREADS && THREADS % XROW == 0 && (ITEMS % THREADS == 0 || XPT == 1), "x items");
 };
 
 __device__ __forceinline__ void cluster_sync()
@@ -293,7 +295,7 @@ __device__ __forceinline__ uint32_t byte_pair(uint32_t a, uint32_t b, int s)
 }
 
 template <typename T, int MT, int NA>
-__global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
+__global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
     k_q4_tc(const __grid_constant__ Q4Args<T> a, const __grid_constant__ CUtensorMap codes_map,
             const __grid_constant__ CUtensorMap x_map, int per, int vec, uint32_t group_magic, uint32_t *err)
 {
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const bool mma_warp = warp == WARPS, tma_warp = warp == WARPS + 1, expands = warp < WARPS;
-    const int half = expands ? warp >> 3 : 0;  // this thread's weight tile
+    const int half = expands && NA == 2 ? warp >> 3 : 0;  // this thread's weight tile
     const int n0 = (blockIdx.x * NA + half) * TC_BM, m0 = blockIdx.y * MT;
     const int nkc = (a.w.K + KC - 1) / KC, c0 = blockIdx.z * per;
     const int nk = nkc - c0 < per ? (nkc - c0 > 0 ? nkc - c0 : 0) : per;
@@ -330,10 +332,10 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    // this thread's units of codes (row, 32 k each) and items of x (row, 8 k each) of every stage
-    const int arow = 16 * (warp & 7) + (lane & 15), aun = lane >> 4;  // units aun, aun + 2
+    // this thread's unit of codes (row, 32 k) and items of x (row, 8 k each) of every stage
+    const int arow = 16 * (warp & 7) + (lane & 15), abox = NA == 1 && S::BOXES == 2 ? warp >> 3 : 0, aun = 2 * abox + (lane >> 4);
     const int xk = tid % S::XROW * 8, xm = tid / S::XROW;
-    const bool has_x = expands && tid < S::ITEMS;
+    const bool has_x = expands && tid < S::ITEMS, has_codes = expands && tid < S::UNITS;
     const int units = (a.w.K + 31) / 32;
     T sum[S::XPT];
 #pragma unroll
@@ -348,13 +350,12 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
     // what lies outside the matrices arrives as zeros
     auto issue = [&](int c, int r) {
         const uint32_t ro = uint32_t(r) * S::RAW;
-#pragma unroll
-        for (int i = 0; i < S::UPT; i++) {
-            const int u = KC / 32 * c + aun + 2 * i;
+        if (has_codes) {
+            const int u = KC / 32 * c + aun;
             const bool in = u < units && n0 + arow < a.w.N;
             const int64_t at = in ? step_at(u) : 0;
             // the aligned pair of steps that holds this one (only its own half at the array's end)
-            cp_async<4>(raw_steps + ro + i * THREADS * 4, a.w.step + (at & ~int64_t(1)), in ? (at & 1 ? 4 : 2) : 0);
+            cp_async<4>(raw_steps + ro, a.w.step + (at & ~int64_t(1)), in ? (at & 1 ? 4 : 2) : 0);
         }
         if (has_x && !vec) {
 #pragma unroll
@@ -375,15 +376,13 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
     auto store_stage = [&](int c, int r, int st) {
         uint8_t *const base = smem + st * S::STAGE;
         const uint8_t *const rp = raw + uint32_t(r) * S::RAW;
-#pragma unroll
-        for (int i = 0; i < S::UPT; i++) {
+        if (has_codes) {
             const uint4 code =
-                *reinterpret_cast<const uint4 *>(rp + i * S::RAW_BOX + (half * TC_BM + arow) * 32 + aun * 16);
-            const uint32_t odd = uint32_t(step_at(KC / 32 * c + aun + 2 * i)) & 1;
-            const uint32_t step =
-                (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + (i * THREADS + tid) * 4) >> (16 * odd)) & Q4_STEP_MAX;
+                *reinterpret_cast<const uint4 *>(rp + abox * S::RAW_BOX + (half * TC_BM + arow) * 32 + (lane >> 4) * 16);
+            const uint32_t odd = uint32_t(step_at(KC / 32 * c + aun)) & 1;
+            const uint32_t step = (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + tid * 4) >> (16 * odd)) & Q4_STEP_MAX;
             const uint32_t bias = (0x8000u - 8u * step) * 0x10001u;
-            uint8_t *const pa = base + half * S::A_TILE + (aun + 2 * i) * 4 * QT_A_CHUNK + arow * 16;
+            uint8_t *const pa = base + half * S::A_TILE + aun * 4 * QT_A_CHUNK + arow * 16;
             *reinterpret_cast<uint4 *>(pa) = q4_expand(code.x, step, bias);
             *reinterpret_cast<uint4 *>(pa + QT_A_CHUNK) = q4_expand(code.y, step, bias);
             *reinterpret_cast<uint4 *>(pa + 2 * QT_A_CHUNK) = q4_expand(code.z, step, bias);
@@ -454,9 +453,9 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
             if (c >= S::RD) ok = mbar_wait(&raw_empty[r], uint32_t((c / S::RD - 1) & 1));
             if (ok && leader) {
                 const uint32_t ra = smem_addr(raw) + uint32_t(r) * S::RAW;
-                mbar_expect(&raw_full[r], S::UPT * S::RAW_BOX + (vec ? MT * KC * P : 0));
+                mbar_expect(&raw_full[r], S::BOXES * S::RAW_BOX + (vec ? MT * KC * P : 0));
 #pragma unroll
-                for (int i = 0; i < S::UPT; i++)
+                for (int i = 0; i < S::BOXES; i++)
                     tma_load_2d(ra + i * S::RAW_BOX, &codes_map, (c0 + c) * (KC / 2) + 32 * i, n0, &raw_full[r]);
                 if (vec) tma_load_2d(ra + S::RAW_X, &x_map, (c0 + c) * KC, m0, &raw_full[r]);
             }
@@ -503,12 +502,12 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
     T *const part = reinterpret_cast<T *>(smem);  // [MT][NA * 128]
     constexpr int PITCH = NA * TC_BM;
     if (all_ok && expands) {
-        const int q = warp & 3, h = (warp >> 2) & 1, nl = half * TC_BM + 32 * q + lane;
+        constexpr int CW = MT < 8 ? MT : 8, GROUPS = WARPS / (4 * NA);  // rows of x per pass; warps per TMEM quarter
+        const int q = warp & 3, h = (warp >> 2) % GROUPS, nl = half * TC_BM + 32 * q + lane;
         const uint32_t lanes = tmem + half * S::NB + (uint32_t(32 * q) << 16);
-        constexpr int CW = MT < 8 ? MT : 8, STEP = MT < 16 ? CW : 2 * CW;  // rows per TMEM pass; narrow tiles: warps 0-3
-        if (MT >= 16 || h == 0) {
+        {
 #pragma unroll 1
-            for (int m = MT < 16 ? 0 : h * CW; m < MT; m += STEP) {
+            for (int m = h * CW; m < MT; m += GROUPS * CW) {
                 uint32_t v[P][8];
                 if constexpr (MT >= 8) {
 #pragma unroll
@@ -545,7 +544,7 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
     if (expands && all_ok) {
         const int parts = int(gridDim.z), rank = int(blockIdx.z);
         const int nl = tid % PITCH, n = blockIdx.x * PITCH + nl;
-        constexpr int ROWS = THREADS / PITCH, U = 8;  // rows per pass; passes per batch
+        constexpr int ROWS = THREADS / PITCH, U = MT / ROWS < 1 ? 1 : MT / ROWS < 8 ? MT / ROWS : 8;  // rows per pass; passes per batch
         if (n < a.w.N) {
             const T bias = a.bias ? __ldg(a.bias + n) : T(0);
             for (int mb = rank * ROWS + tid / PITCH; mb < MT; mb += U * ROWS * parts) {
@@ -555,14 +554,15 @@ __global__ void __launch_bounds__(NA *Q4_THREADS + 64, QtShape<T, MT, NA>::CTAS)
                     const int m = mb + i * ROWS * parts;
                     const bool in = m < MT && m0 + m < a.M;
                     add[i] = in && a.Add ? a.Add[int64_t(m0 + m) * a.w.N + n] : T(0);
-                    v[i] = 0;
-                    if (in) {
-                        if (parts == 1)
-                            v[i] = part[m * PITCH + nl];
-                        else
-                            for (int z = 0; z < parts; z++) v[i] += ld_cluster(part + m * PITCH + nl, z);
-                    }
+                    v[i] = parts == 1 && m < MT ? part[m * PITCH + nl] : T(0);
                 }
+                if (parts > 1)
+                    for (int z = 0; z < parts; z++)
+#pragma unroll
+                        for (int i = 0; i < U; i++) {
+                            const int m = mb + i * ROWS * parts;
+                            if (m < MT) v[i] += ld_cluster(part + m * PITCH + nl, z);
+                        }
 #pragma unroll
                 for (int i = 0; i < U; i++) {
                     const int m = mb + i * ROWS * parts;
@@ -660,7 +660,19 @@ static int launch_gemv(const Q4Args<T> &a, cudaStream_t st)
     return DDG_OK;
 }
 
-template <typename T, int MT, int NA = 1>
+// CTAs of a cluster that K is split over: while that leaves every CTA resident
+// at once and two stages each, and for as long as a CTA's sums need it.
+// Clusters of four: of eight, only 15 fit the device at a time (256 CTAs of a
+// 4 x 4096 x 4096 product took three rounds).
+static int qt_split(int kc, int na, int K, int64_t ctas)
+{
+    int split = 1;
+    while (na == 1 && split < 4 && ctas * split * 2 <= 148 && K >= 4 * kc * split) split *= 2;
+    while (na == 1 && split < 8 && int64_t(K) > int64_t(QT_MAX_K) * split) split *= 2;
+    return split;
+}
+
+template <typename T, int MT, int NA>
 static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
 {
     using S = QtShape<T, MT, NA>;
@@ -672,13 +684,8 @@ static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
     const int nkc = (a.w.K + S::KC - 1) / S::KC;
     const int64_t gn = (int64_t(a.w.N) + NA * TC_BM - 1) / (NA * TC_BM), gm = (int64_t(a.M) + MT - 1) / MT;
     DDG_CHECK(gm <= 65535, DDG_ERR_ARG, "fc_q4: %d rows are too many for one call", a.M);
-    // K split over a cluster while that leaves every CTA resident at once and two
-    // stages each.  Clusters of four: of eight, only 15 fit the device at a time
-    // (256 CTAs of a 4 x 4096 x 4096 product took three rounds).
-    int split = 1;
-    while (NA == 1 && split < 4 && gn * gm * split * 2 <= S::CTAS * 148 && nkc >= 4 * split) split *= 2;
+    const int split = qt_split(S::KC, NA, a.w.K, gn * gm);
     const int most = QT_MAX_K / S::KC;
-    while (NA == 1 && split < 8 && nkc > most * split) split *= 2;
     DDG_CHECK(nkc <= most * split, DDG_ERR_ARG, "fc_q4: K = %d is too long (at most %d)", a.w.K, 8 * QT_MAX_K);
     const int per = nkc ? (nkc + split - 1) / split : 1;
     const int vec = q4_vec(a);
@@ -715,24 +722,32 @@ int fc_q4(const Q4Args<T> &a, cudaStream_t st)
     const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
     if (a.M <= 2 && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
         return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
-    // the fewest rows per tile that hold them all, up to 256 MMA columns; two
-    // weight tiles per CTA where those alone give every SM one (each split of x
-    // then serves 256 outputs), and K needs no split for the sums' range
-    constexpr int MT = 256 / int(sizeof(T));
-    const bool wide = (int64_t(a.w.N) + 255) / 256 * ((int64_t(a.M) + MT - 1) / MT) >= 148 && a.w.K <= QT_MAX_K;
-    if constexpr (sizeof(T) == 4) {
-        if (a.M <= 4) return launch_tc_q4<T, 4>(a, st);
-        if (a.M <= 8) return launch_tc_q4<T, 8>(a, st);
-        if (a.M <= 16) return launch_tc_q4<T, 16>(a, st);
-        if (a.M <= 32) return launch_tc_q4<T, 32>(a, st);
-        return wide ? launch_tc_q4<T, 64, 2>(a, st) : launch_tc_q4<T, 64>(a, st);
-    } else {
-        if (a.M <= 2) return launch_tc_q4<T, 2>(a, st);
-        if (a.M <= 4) return launch_tc_q4<T, 4>(a, st);
-        if (a.M <= 8) return launch_tc_q4<T, 8>(a, st);
-        if (a.M <= 16) return launch_tc_q4<T, 16>(a, st);
-        return wide ? launch_tc_q4<T, 32, 2>(a, st) : launch_tc_q4<T, 32>(a, st);
+    // The tile of least estimated time.  Wide tiles expand the weights fewer times
+    // and split x for more outputs, narrow ones spread a small product over more
+    // SMs: 256 x 1024 x 512 takes 7.9 us in tiles of 16 rows and 9.8 in tiles of
+    // 64; 256 x 4096 x 8192 takes 103 us in tiles of 64 rows by 128 outputs and 59
+    // by 256.  Stage times (us per 64 k) are fits to such measurements.
+    constexpr int F = sizeof(T) / 4;
+    struct Tile {
+        int mt, na, kc;
+        double us;
+        int (*launch)(const Q4Args<T> &, cudaStream_t);
+    };
+    static const Tile tiles[] = {{4 / F, 1, 128, 0.22, launch_tc_q4<T, 4 / F, 1>},   {8 / F, 1, 128, 0.24, launch_tc_q4<T, 8 / F, 1>},
+                                 {16 / F, 1, 128, 0.28, launch_tc_q4<T, 16 / F, 1>}, {32 / F, 1, 128, 0.42, launch_tc_q4<T, 32 / F, 1>},
+                                 {64 / F, 1, 64, 0.70, launch_tc_q4<T, 64 / F, 1>},  {64 / F, 2, 64, 0.90, launch_tc_q4<T, 64 / F, 2>}};
+    const Tile *best = nullptr;
+    double least = 0;
+    for (const Tile &t : tiles) {
+        const int64_t ctas = (int64_t(a.w.N) + t.na * TC_BM - 1) / (t.na * TC_BM) * ((int64_t(a.M) + t.mt - 1) / t.mt);
+        const int split = qt_split(t.kc, t.na, a.w.K, ctas);
+        const double rounds = double((ctas * split + 147) / 148);
+        const double us = rounds * (2.0 + t.us * double((a.w.K + 63) / 64) / split);
+        const bool fits = (int64_t(a.w.K) + split - 1) / split <= QT_MAX_K && (int64_t(a.M) + t.mt - 1) / t.mt <= 65535;
+        if (fits && (!best || us < least)) best = &t, least = us;
     }
+    DDG_CHECK(best, DDG_ERR_ARG, "fc_q4: %d rows of K = %d are too many for one call", a.M, a.w.K);
+    return best->launch(a, st);
 }
 template int fc_q4<uint32_t>(const Q4Args<uint32_t> &, cudaStream_t);
 template int fc_q4<uint64_t>(const Q4Args<uint64_t> &, cudaStream_t);
