@@ -217,7 +217,6 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
 
 // ------------------------------------------------------------------ more rows: tensor cores
 
-constexpr int QT_STAGES = 2;
 constexpr int QT_MAX_K = 32768;            // k per CTA: a column's sum, 2 * 255^2 * K, stays below 2^32
 // operands lie in 16-byte chunks of 8 k, chunk-major: rows 16 bytes apart,
 // chunks of A 2048 and of B 16 NB + 16 bytes apart (the pad spreads the chunks
@@ -235,10 +234,15 @@ struct QtShape {
     static constexpr int BOXES = KC / 64;                          // 32-byte boxes of codes per row and stage
     // sixteen warps to expand; a unit of codes for each thread of the first UNITS
     static constexpr int THREADS = 512, UNITS = NA * BOXES * 256;
+    static constexpr int NST = NB <= 64 ? 3 : 2;                   // stages of planes
     static constexpr int CH = KC / 8, XROW = KC / 8;               // chunks per stage; x items of 8 k per row
-    static constexpr int COLS = tmem_cols(NA * NB);
+    // one weight tile goes straight to tensor memory (KC / 2 columns a stage), which
+    // spares the shared memory half of its traffic; beside two tiles' 512
+    // accumulator columns there is no room for it
+    static constexpr bool A_TMEM = NA == 1;
+    static constexpr int A_COLS = A_TMEM ? KC / 2 : 0, COLS = tmem_cols(NA * NB + NST * A_COLS);
     static constexpr uint32_t B_CHUNK = NB * 16 + 16;
-    static constexpr uint32_t A_TILE = CH * QT_A_CHUNK, A_STAGE = NA * A_TILE, STAGE = A_STAGE + CH * B_CHUNK;
+    static constexpr uint32_t A_TILE = CH * QT_A_CHUNK, A_STAGE = A_TMEM ? 0 : NA * A_TILE, STAGE = A_STAGE + CH * B_CHUNK;
     static constexpr int ITEMS = MT * XROW, XPT = (ITEMS + THREADS - 1) / THREADS;
     // A stage's codes (BOXES of 32 bytes a row), x and steps as they lie in
     // memory, loaded RD stages ahead: the memory needs about 40 KB of codes in
@@ -246,12 +250,12 @@ struct QtShape {
     // expanding threads took 600-1000 cycles a stage to issue.)
     static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = BOXES * RAW_BOX, RAW_STEPS = RAW_X + MT * KC * P;
     static constexpr uint32_t RAW = RAW_STEPS + UNITS * 4;
-    static constexpr int RD_FIT = int((212 * 1024 - QT_STAGES * STAGE) / RAW);
+    static constexpr int RD_FIT = int((212 * 1024 - NST * STAGE) / RAW);
     static constexpr int RD = RD_FIT < 2 ? 2 : RD_FIT > 8 ? 8 : RD_FIT;
     // [barriers, TMEM address | sums of x | pad to 1024 | stages | raw stages | slack]
     static constexpr uint32_t HEAD = 256 + MT * P;
     static constexpr uint32_t XPITCH = (ITEMS < THREADS ? ITEMS : THREADS) * 16;  // between 16-byte pieces of the x items
-    static constexpr uint32_t SMEM = HEAD + 1024 + QT_STAGES * STAGE + RD * RAW + 2048;
+    static constexpr uint32_t SMEM = HEAD + 1024 + NST * STAGE + RD * RAW + 2048;
     static_assert(NB % 16 == 0 && NB <= 256 && STAGE % 128 == 0 && RAW % 128 == 0 && RAW_X % 128 == 0, "tile");
     static_assert(UNITS <= THREADS && THREADS % XROW == 0 && (ITEMS % THREADS == 0 || XPT == 1), "x items");
 };
@@ -300,10 +304,10 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
             const __grid_constant__ CUtensorMap x_map, int per, int vec, uint32_t group_magic, uint32_t *err)
 {
     using S = QtShape<T, MT, NA>;
-    constexpr int P = S::P, THREADS = S::THREADS, KC = S::KC, WARPS = THREADS / 32;
+    constexpr int P = S::P, THREADS = S::THREADS, KC = S::KC, WARPS = THREADS / 32, NST = S::NST;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint64_t *const empty = reinterpret_cast<uint64_t *>(smem_raw), *const full = empty + QT_STAGES;
-    uint64_t *const raw_full = full + QT_STAGES, *const raw_empty = raw_full + 8;  // (2 + 2 + 8 + 8) x 8 bytes
+    uint64_t *const empty = reinterpret_cast<uint64_t *>(smem_raw), *const full = empty + NST;
+    uint64_t *const raw_full = full + NST, *const raw_empty = raw_full + 8;  // (3 + 3 + 8 + 8) x 8 bytes
     uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(smem_raw + 192);
     T *const xsum = reinterpret_cast<T *>(smem_raw + 256);  // [MT]
     uint8_t *const smem = smem_raw + S::HEAD + ((1024u - ((smem_addr(smem_raw) + S::HEAD) & 1023u)) & 1023u);
@@ -322,7 +326,7 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < QT_STAGES; i++) mbar_init(empty + i, 1), mbar_init(full + i, WARPS);
+        for (int i = 0; i < NST; i++) mbar_init(empty + i, 1), mbar_init(full + i, WARPS);
         for (int i = 0; i < S::RD; i++) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, WARPS);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -333,14 +337,16 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
     const uint32_t tmem = s_tmem;
 
     // this thread's unit of codes (row, 32 k) and items of x (row, 8 k each) of every stage
-    const int arow = 16 * (warp & 7) + (lane & 15), abox = NA == 1 && S::BOXES == 2 ? warp >> 3 : 0, aun = 2 * abox + (lane >> 4);
+    // (in tensor memory a warp reaches the rows of its quarter only)
+    const int arow = S::A_TMEM ? 32 * (warp & 3) + lane : 16 * (warp & 7) + (lane & 15);
+    const int aun = S::A_TMEM ? warp >> 2 : lane >> 4;
     const int xk = tid % S::XROW * 8, xm = tid / S::XROW;
     const bool has_x = expands && tid < S::ITEMS, has_codes = expands && tid < S::UNITS;
     const int units = (a.w.K + 31) / 32;
     T sum[S::XPT];
 #pragma unroll
     for (int i = 0; i < S::XPT; i++) sum[i] = 0;
-    uint8_t *const raw = smem + QT_STAGES * S::STAGE;
+    uint8_t *const raw = smem + NST * S::STAGE;
     const uint32_t raw_steps = smem_addr(raw) + S::RAW_STEPS + 4 * tid, raw_x = smem_addr(raw) + S::RAW_X + 16 * tid;
     // index of the step of unit u of a row: u / (group / 32), by the exact reciprocal (u < 2^13)
     auto step_at = [&](int u) {
@@ -377,16 +383,24 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         uint8_t *const base = smem + st * S::STAGE;
         const uint8_t *const rp = raw + uint32_t(r) * S::RAW;
         if (has_codes) {
-            const uint4 code =
-                *reinterpret_cast<const uint4 *>(rp + abox * S::RAW_BOX + (half * TC_BM + arow) * 32 + (lane >> 4) * 16);
+            const uint4 code = *reinterpret_cast<const uint4 *>(rp + (aun >> 1) * S::RAW_BOX + (half * TC_BM + arow) * 32 +
+                                                                (aun & 1) * 16);
             const uint32_t odd = uint32_t(step_at(KC / 32 * c + aun)) & 1;
-            const uint32_t step = (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + tid * 4) >> (16 * odd)) & Q4_STEP_MAX;
+            const uint32_t step =
+                (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + tid * 4) >> (16 * odd)) & Q4_STEP_MAX;
             const uint32_t bias = (0x8000u - 8u * step) * 0x10001u;
-            uint8_t *const pa = base + half * S::A_TILE + aun * 4 * QT_A_CHUNK + arow * 16;
-            *reinterpret_cast<uint4 *>(pa) = q4_expand(code.x, step, bias);
-            *reinterpret_cast<uint4 *>(pa + QT_A_CHUNK) = q4_expand(code.y, step, bias);
-            *reinterpret_cast<uint4 *>(pa + 2 * QT_A_CHUNK) = q4_expand(code.z, step, bias);
-            *reinterpret_cast<uint4 *>(pa + 3 * QT_A_CHUNK) = q4_expand(code.w, step, bias);
+            const uint4 w[4] = {q4_expand(code.x, step, bias), q4_expand(code.y, step, bias), q4_expand(code.z, step, bias),
+                                q4_expand(code.w, step, bias)};
+            if constexpr (S::A_TMEM) {
+                const uint32_t v[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
+                                        w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
+                tc_fence_after();  // the MMAs that read this stage are done
+                tmem_st16(tmem + (uint32_t(32 * (warp & 3)) << 16) + NA * S::NB + st * S::A_COLS + aun * 16, v);
+            } else {
+                uint8_t *const pa = base + half * S::A_TILE + aun * 4 * QT_A_CHUNK + arow * 16;
+#pragma unroll
+                for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(pa + i * QT_A_CHUNK) = w[i];
+            }
         }
         if (has_x) {
 #pragma unroll
@@ -430,18 +444,25 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
     if (mma_warp) {
         const bool leader = elect_one();
         for (int c = 0; c < nk && ok; c++) {
-            const int st = c % QT_STAGES;
-            ok = mbar_wait(&full[st], uint32_t((c / QT_STAGES) & 1));
+            const int st = c % NST;
+            ok = mbar_wait(&full[st], uint32_t((c / NST) & 1));
             tc_fence_after();
             if (ok && leader) {
+                // descriptors step by constants in their address field (16-byte units)
                 const uint32_t sa = smem_addr(smem + st * S::STAGE), sb = sa + S::A_STAGE;
+                const uint64_t db = smem_desc(sb, S::B_CHUNK, 128), da = smem_desc(sa, QT_A_CHUNK, 128);
+                const uint32_t ta = tmem + S::NB + st * S::A_COLS;
 #pragma unroll
                 for (int h = 0; h < KC / 16; h++) {
-                    const uint64_t db = smem_desc(sb + h * 2 * S::B_CHUNK, S::B_CHUNK, 128);
 #pragma unroll
-                    for (int t = 0; t < NA; t++)
-                        mma_i8(tmem + t * S::NB, smem_desc(sa + t * S::A_TILE + h * 2 * QT_A_CHUNK, QT_A_CHUNK, 128), db,
-                               IDESC, (c > 0 || h > 0) ? 1u : 0u);
+                    for (int t = 0; t < NA; t++) {
+                        const uint64_t dbh = db + uint64_t(h * 2 * S::B_CHUNK >> 4);
+                        if constexpr (S::A_TMEM)
+                            mma_i8_ts(tmem, ta + h * 8, dbh, IDESC, (c > 0 || h > 0) ? 1u : 0u);
+                        else
+                            mma_i8(tmem + t * S::NB, da + uint64_t((t * S::A_TILE + h * 2 * QT_A_CHUNK) >> 4), dbh, IDESC,
+                                   (c > 0 || h > 0) ? 1u : 0u);
+                    }
                 }
                 mma_commit(&empty[st]);
             }
@@ -471,10 +492,10 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
                 cp_async_commit();
         }
         for (int c = 0, r = 0; c < nk; c++, r = r + 1 == S::RD ? 0 : r + 1) {
-            const int st = c % QT_STAGES;
+            const int st = c % NST;
             cp_async_wait<S::RD - 1>();  // this thread's copies of stage c have landed
             ok = mbar_wait(&raw_full[r], uint32_t((c / S::RD) & 1));
-            if (ok && c >= QT_STAGES) ok = mbar_wait(&empty[st], uint32_t((c / QT_STAGES - 1) & 1));
+            if (ok && c >= NST) ok = mbar_wait(&empty[st], uint32_t((c / NST - 1) & 1));
             if (!__all_sync(0xffffffffu, ok)) break;
             store_stage(c0 + c, r, st);
             if (c + S::RD < nk)
@@ -482,13 +503,17 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
             else
                 cp_async_commit();
             proxy_fence();
+            if constexpr (S::A_TMEM) {
+                tmem_st_wait();
+                tc_fence_before();
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[st]), mbar_arrive(&raw_empty[r]);
         }
         cp_async_wait<0>();
     }
     // the last stage's commit covers every MMA before it
-    if (ok && nk > 0) ok = mbar_wait(&empty[(nk - 1) % QT_STAGES], uint32_t(((nk - 1) / QT_STAGES) & 1));
+    if (ok && nk > 0) ok = mbar_wait(&empty[(nk - 1) % NST], uint32_t(((nk - 1) / NST) & 1));
     if (has_x) {
         using U = std::conditional_t<P == 4, unsigned int, unsigned long long>;
 #pragma unroll

@@ -321,11 +321,11 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
                 tc_fence_after();
                 if (ok && leader) {
                     const uint32_t sa = smem_addr(smem + st * S::STAGE);
-                    const uint64_t db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
+                    const uint64_t da = smem_desc(sa, 128, S::SBO), db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
 #pragma unroll
-                    for (int i = 0; i < P; i++)
-                        mma_i8(tmem + uint32_t(i * NT), smem_desc(sa + i * S::A_PLANE, 128, S::SBO), db,
-                               i8_idesc((P - i) * NT, false), (s > 0 || i > 0) ? 1u : 0u);
+                    for (int i = 0; i < P; i++)  // the address field counts 16-byte units
+                        mma_i8(tmem + uint32_t(i * NT), da + uint64_t(i * S::A_PLANE >> 4), db, i8_idesc((P - i) * NT, false),
+                               (s > 0 || i > 0) ? 1u : 0u);
                     mma_commit(&empty[st]);
                 }
                 __syncwarp();
