@@ -6,13 +6,13 @@
 // Two kernels, both exact modulo 2^bw, so the result does not depend on how K
 // is split over lanes, warps or CTAs.
 //
-// k_q4_gemv, for one or two rows: 8-bit limb products on the CUDA cores.  x
+// k_q4_gemv, for one or two rows of a small product: 8-bit limb products on the CUDA cores.  x
 // sits in shared memory as byte planes, four k of one limb to a word, and
 // dp4a multiplies a word by four codes: per unit of 32 codes (one 16-byte
 // load, one step)
 //   sum_k x_k W_k = step * ( sum_l 2^(8l) dp4a(code, limb l of x) - 8 sum_k x_k ).
 //
-// k_q4_tc, for more rows: the weights are 16-bit numbers, W + 2^15 = w0 + 2^8 w1
+// k_q4_tc, for everything else: the weights are 16-bit numbers, W + 2^15 = w0 + 2^8 w1
 // with unsigned bytes, and x = sum_l 2^(8l) x_l, so
 //   x . W = sum_s 2^(8s) sum_k (w0 x_s + w1 x_{s-1})  -  2^15 sum_k x_k .
 // The weights are the M side of the MMA (128 outputs) as they are, two bytes a
@@ -244,12 +244,11 @@ struct QtShape {
     static constexpr uint32_t B_CHUNK = NB * 16 + 16;
     static constexpr uint32_t A_TILE = CH * QT_A_CHUNK, A_STAGE = A_TMEM ? 0 : NA * A_TILE, STAGE = A_STAGE + CH * B_CHUNK;
     static constexpr int ITEMS = MT * XROW, XPT = (ITEMS + THREADS - 1) / THREADS;
-    // A stage's codes (BOXES of 32 bytes a row), x and steps as they lie in
+    // A stage's codes (BOXES of 32 bytes a row) and x as they lie in
     // memory, loaded RD stages ahead: the memory needs about 40 KB of codes in
     // flight per SM for its latency.  (Asynchronous 16-byte copies by the
     // expanding threads took 600-1000 cycles a stage to issue.)
-    static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = BOXES * RAW_BOX, RAW_STEPS = RAW_X + MT * KC * P;
-    static constexpr uint32_t RAW = RAW_STEPS + UNITS * 4;
+    static constexpr uint32_t RAW_BOX = NA * TC_BM * 32, RAW_X = BOXES * RAW_BOX, RAW = RAW_X + MT * KC * P;
     static constexpr int RD_FIT = int((212 * 1024 - NST * STAGE) / RAW);
     static constexpr int RD = RD_FIT < 2 ? 2 : RD_FIT > 8 ? 8 : RD_FIT;
     // [barriers, TMEM address | sums of x | pad to 1024 | stages | raw stages | slack]
@@ -347,22 +346,19 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
 #pragma unroll
     for (int i = 0; i < S::XPT; i++) sum[i] = 0;
     uint8_t *const raw = smem + NST * S::STAGE;
-    const uint32_t raw_steps = smem_addr(raw) + S::RAW_STEPS + 4 * tid, raw_x = smem_addr(raw) + S::RAW_X + 16 * tid;
-    // index of the step of unit u of a row: u / (group / 32), by the exact reciprocal (u < 2^13)
-    auto step_at = [&](int u) {
-        return int64_t(group_magic ? __umulhi(uint32_t(u), group_magic) : uint32_t(u)) * a.w.N + n0 + arow;
+    const uint32_t raw_x = smem_addr(raw) + S::RAW_X + 16 * tid;
+    // step of this thread's unit of stage c: unit u's is u / (group / 32), by the exact reciprocal (u < 2^13)
+    const bool step_row = has_codes && n0 + arow < a.w.N;
+    const uint16_t *const step_col = a.w.step + n0 + arow;
+    auto step_of = [&](int c) -> uint32_t {
+        const int u = KC / 32 * c + aun;
+        const uint32_t g = group_magic ? __umulhi(uint32_t(u), group_magic) : uint32_t(u);
+        return step_row && u < units ? __ldg(step_col + int64_t(g) * a.w.N) : 0;
     };
-    // copies stage c's steps into raw stage r (and x where its rows are not on 16-byte boundaries);
-    // what lies outside the matrices arrives as zeros
+    // x of stage c into raw stage r where its rows are not on 16-byte boundaries; what lies outside the matrix
+    // arrives as zeros
     auto issue = [&](int c, int r) {
         const uint32_t ro = uint32_t(r) * S::RAW;
-        if (has_codes) {
-            const int u = KC / 32 * c + aun;
-            const bool in = u < units && n0 + arow < a.w.N;
-            const int64_t at = in ? step_at(u) : 0;
-            // the aligned pair of steps that holds this one (only its own half at the array's end)
-            cp_async<4>(raw_steps + ro, a.w.step + (at & ~int64_t(1)), in ? (at & 1 ? 4 : 2) : 0);
-        }
         if (has_x && !vec) {
 #pragma unroll
             for (int j = 0; j < S::XPT; j++) {
@@ -379,15 +375,13 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         cp_async_commit();
     };
     // expands raw stage r into the planes of stage st
-    auto store_stage = [&](int c, int r, int st) {
+    auto store_stage = [&](int r, int st, uint32_t step) {
         uint8_t *const base = smem + st * S::STAGE;
         const uint8_t *const rp = raw + uint32_t(r) * S::RAW;
         if (has_codes) {
             const uint4 code = *reinterpret_cast<const uint4 *>(rp + (aun >> 1) * S::RAW_BOX + (half * TC_BM + arow) * 32 +
                                                                 (aun & 1) * 16);
-            const uint32_t odd = uint32_t(step_at(KC / 32 * c + aun)) & 1;
-            const uint32_t step =
-                (*reinterpret_cast<const uint32_t *>(rp + S::RAW_STEPS + tid * 4) >> (16 * odd)) & Q4_STEP_MAX;
+            step &= Q4_STEP_MAX;
             const uint32_t bias = (0x8000u - 8u * step) * 0x10001u;
             const uint4 w[4] = {q4_expand(code.x, step, bias), q4_expand(code.y, step, bias), q4_expand(code.z, step, bias),
                                 q4_expand(code.w, step, bias)};
@@ -471,6 +465,8 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
     } else if (tma_warp) {
         const bool leader = elect_one();
         for (int c = 0, r = 0; c < nk && ok; c++, r = r + 1 == S::RD ? 0 : r + 1) {
+            // (not the full barriers: between two uses of a raw stage they can pass two phases, and a parity
+            // tells only neighbouring ones apart)
             if (c >= S::RD) ok = mbar_wait(&raw_empty[r], uint32_t((c / S::RD - 1) & 1));
             if (ok && leader) {
                 const uint32_t ra = smem_addr(raw) + uint32_t(r) * S::RAW;
@@ -485,23 +481,28 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         // nobody leaves with copies in flight
         if (ok && nk > 0) ok = mbar_wait(&raw_full[(nk - 1) % S::RD], uint32_t(((nk - 1) / S::RD) & 1));
     } else {
-        for (int c = 0; c < S::RD; c++) {
-            if (c < nk)
-                issue(c0 + c, c);
-            else
-                cp_async_commit();
-        }
+        if (!vec)
+            for (int c = 0; c < S::RD; c++) {
+                if (c < nk)
+                    issue(c0 + c, c);
+                else
+                    cp_async_commit();
+            }
+        uint32_t step = nk > 0 ? step_of(c0) : 0;
         for (int c = 0, r = 0; c < nk; c++, r = r + 1 == S::RD ? 0 : r + 1) {
             const int st = c % NST;
-            cp_async_wait<S::RD - 1>();  // this thread's copies of stage c have landed
+            if (!vec) cp_async_wait<S::RD - 1>();  // this thread's copies of stage c have landed
             ok = mbar_wait(&raw_full[r], uint32_t((c / S::RD) & 1));
             if (ok && c >= NST) ok = mbar_wait(&empty[st], uint32_t((c / NST - 1) & 1));
             if (!__all_sync(0xffffffffu, ok)) break;
-            store_stage(c0 + c, r, st);
-            if (c + S::RD < nk)
-                issue(c0 + c + S::RD, r);
-            else
-                cp_async_commit();
+            store_stage(r, st, step);
+            if (c + 1 < nk) step = step_of(c0 + c + 1);
+            if (!vec) {
+                if (c + S::RD < nk)
+                    issue(c0 + c + S::RD, r);
+                else
+                    cp_async_commit();
+            }
             proxy_fence();
             if constexpr (S::A_TMEM) {
                 tmem_st_wait();
@@ -745,7 +746,10 @@ int fc_q4(const Q4Args<T> &a, cudaStream_t st)
         return DDG_OK;
     }
     const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
-    if (a.M <= 2 && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
+    // the CUDA cores for one or two rows while the product is small: 1 x 1024 x 1024 takes 4.4 us there and
+    // 5.6 on the tensor cores, 1 x 4096 x 4096 over Z_2^64 13.8 and 10.7
+    const uint64_t macs = uint64_t(a.M) * uint64_t(a.w.K) * uint64_t(a.w.N);
+    if (a.M <= 2 && macs * sizeof(T) <= (1u << 25) && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
         return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
     // The tile of least estimated time.  Wide tiles expand the weights fewer times
     // and split x for more outputs, narrow ones spread a small product over more
