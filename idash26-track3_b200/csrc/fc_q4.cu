@@ -433,6 +433,24 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         }
     };
 
+    // this thread's outputs, and the first ones' Add and bias on their way while the products are formed
+    constexpr int PITCH = NA * TC_BM, ROWS = THREADS / PITCH;                    // outputs per row of x, rows per pass
+    constexpr int U = MT / ROWS < 1 ? 1 : MT / ROWS < 8 ? MT / ROWS : 8;         // passes per batch
+    const int parts = int(gridDim.z), pitch_m = ROWS * parts;
+    const int ol = tid % PITCH, on = blockIdx.x * PITCH + ol, om = int(blockIdx.z) * ROWS + tid / PITCH;
+    T add[U], bias = 0;
+    auto load_add = [&](int mb) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int m = mb + i * pitch_m;
+            add[i] = a.Add && on < a.w.N && m < MT && m0 + m < a.M ? a.Add[int64_t(m0 + m) * a.w.N + on] : T(0);
+        }
+    };
+    if (expands) {
+        load_add(om);
+        if (a.bias && on < a.w.N) bias = __ldg(a.bias + on);
+    }
+
     constexpr uint32_t IDESC = i8_idesc(S::NB, false);
     bool ok = true;
     if (mma_warp) {
@@ -464,6 +482,7 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         }
     } else if (tma_warp) {
         const bool leader = elect_one();
+        if (leader) tma_prefetch(&codes_map), tma_prefetch(&x_map);
         for (int c = 0, r = 0; c < nk && ok; c++, r = r + 1 == S::RD ? 0 : r + 1) {
             // (not the full barriers: between two uses of a raw stage they can pass two phases, and a parity
             // tells only neighbouring ones apart)
@@ -525,8 +544,7 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
 
     // this CTA's sums of (row m, output n) to shared memory (the stages are done), all of them added up
     // over the cluster and written in batches whose loads overlap
-    T *const part = reinterpret_cast<T *>(smem);  // [MT][NA * 128]
-    constexpr int PITCH = NA * TC_BM;
+    T *const part = reinterpret_cast<T *>(smem);  // [MT][PITCH]
     if (all_ok && expands) {
         constexpr int CW = MT < 8 ? MT : 8, GROUPS = WARPS / (4 * NA);  // rows of x per pass; warps per TMEM quarter
         const int q = warp & 3, h = (warp >> 2) % GROUPS, nl = half * TC_BM + 32 * q + lane;
@@ -567,33 +585,28 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         cluster_sync();
     else
         __syncthreads();
-    if (expands && all_ok) {
-        const int parts = int(gridDim.z), rank = int(blockIdx.z);
-        const int nl = tid % PITCH, n = blockIdx.x * PITCH + nl;
-        constexpr int ROWS = THREADS / PITCH, U = MT / ROWS < 1 ? 1 : MT / ROWS < 8 ? MT / ROWS : 8;  // rows per pass; passes per batch
-        if (n < a.w.N) {
-            const T bias = a.bias ? __ldg(a.bias + n) : T(0);
-            for (int mb = rank * ROWS + tid / PITCH; mb < MT; mb += U * ROWS * parts) {
-                T add[U], v[U];
+    if (expands && all_ok && on < a.w.N) {
+        for (int mb = om; mb < MT; mb += U * pitch_m) {
+            T v[U];
 #pragma unroll
-                for (int i = 0; i < U; i++) {
-                    const int m = mb + i * ROWS * parts;
-                    const bool in = m < MT && m0 + m < a.M;
-                    add[i] = in && a.Add ? a.Add[int64_t(m0 + m) * a.w.N + n] : T(0);
-                    v[i] = parts == 1 && m < MT ? part[m * PITCH + nl] : T(0);
-                }
-                if (parts > 1)
-                    for (int z = 0; z < parts; z++)
+            for (int i = 0; i < U; i++) {
+                const int m = mb + i * pitch_m;
+                v[i] = !split && m < MT ? part[m * PITCH + ol] : T(0);
+            }
+            if (split)
+                for (int z = 0; z < parts; z++)
 #pragma unroll
-                        for (int i = 0; i < U; i++) {
-                            const int m = mb + i * ROWS * parts;
-                            if (m < MT) v[i] += ld_cluster(part + m * PITCH + nl, z);
-                        }
+                    for (int i = 0; i < U; i++) {
+                        const int m = mb + i * pitch_m;
+                        if (m < MT) v[i] += ld_cluster(part + m * PITCH + ol, z);
+                    }
 #pragma unroll
-                for (int i = 0; i < U; i++) {
-                    const int m = mb + i * ROWS * parts;
-                    if (m < MT && m0 + m < a.M) a.out[int64_t(m0 + m) * a.w.N + n] = a.sign * v[i] + bias + add[i];
-                }
+            for (int i = 0; i < U; i++) v[i] = a.sign * v[i] + bias + add[i];
+            load_add(mb + U * pitch_m);
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const int m = mb + i * pitch_m;
+                if (m < MT && m0 + m < a.M) a.out[int64_t(m0 + m) * a.w.N + on] = v[i];
             }
         }
     }

@@ -37,6 +37,11 @@ inline int tma_map_2d(CUtensorMap *map, const void *base, int elem_bytes, uint64
     return DDG_OK;
 }
 
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap *map)
+{
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int col, int row, uint64_t *bar)
 {
     asm volatile(
