@@ -656,6 +656,150 @@ __global__ void __launch_bounds__(LT_THREADS + 32, 2)
     la_tiles<T, LT_OUTPUT>(blockIdx.x, gridDim.x, count, tile_of, a.p0, two == 2, a.z, a.out, err);
 }
 
+// ------------------------------------------------------------------ matrix stages of a few heads
+//
+// The same products on the CUDA cores, in 32 x 32 tiles, for calls whose few
+// 128-row tiles would leave most SMs idle and run at one tile's latency.  256
+// threads, four rows of one column each; the next 32 k on their way in registers.
+template <typename T>
+struct LsTile {
+    LtPair<T> p[2];
+    int pairs, rows, cols, i0, j0;  // the product's extent, this tile's corner
+    int64_t at, stride;             // as LtTile, from row 0 and column 0
+};
+
+template <typename T>
+constexpr int LS_W = 32 + VEC<T>;  // row pitch: 16-byte rows for the A reads, off the banks of the next row
+template <typename T, int KIND>
+__device__ __forceinline__ void ls_tile(T (&sm)[4][32][LS_W<T>], const LsTile<T> &t, T p0, bool beaver, const T *z, T *out)
+{
+    // A, [A] (row, k); p0 B - [B], B (k, column)
+    auto &as = sm[0], &am = sm[1], &br = sm[2], &bs = sm[3];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    T acc[4] = {0, 0, 0, 0};
+    T ra[4], rm[4], rb[4], rn[4];
+    auto load = [&](int which, int k0) {
+        const LtPair<T> &p = t.p[which];
+        const bool tri = KIND == LT_OUTPUT && which == 0;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int y4 = y + 8 * q;
+            {  // A: x runs along what is contiguous
+                const int row = t.i0 + (KIND == LT_STATES ? x : y4), k = k0 + (KIND == LT_STATES ? y4 : x);
+                const bool in = row < t.rows && k < p.K && (!tri || k <= row);
+                const int64_t o = KIND == LT_STATES ? k * p.lda + row : tri ? row * (row + 1) / 2 + k : row * p.lda + k;
+                ra[q] = in ? __ldg(p.a + o) : T(0), rm[q] = in && beaver ? __ldg(p.a_ms + o) : T(0);
+            }
+            {
+                const int col = t.j0 + (KIND == LT_SCORES ? y4 : x), k = k0 + (KIND == LT_SCORES ? x : y4);
+                const bool in = col < t.cols && k < p.K;
+                const int64_t o = KIND == LT_SCORES ? col * p.ldb + k : k * p.ldb + col;
+                rb[q] = in ? __ldg(p.b + o) : T(0), rn[q] = in && beaver ? __ldg(p.b_ms + o) : T(0);
+            }
+        }
+    };
+    // entries right of a causal tile's last row add nothing
+    auto length = [&](int which) {
+        const int K = t.p[which].K;
+        return KIND == LT_OUTPUT && which == 0 && t.i0 + 32 < K ? t.i0 + 32 : K;
+    };
+    int which = 0, k0 = 0;
+    load(0, 0);
+    while (which < t.pairs) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int y4 = y + 8 * q;
+            (KIND == LT_STATES ? as[x][y4] : as[y4][x]) = ra[q], (KIND == LT_STATES ? am[x][y4] : am[y4][x]) = rm[q];
+            (KIND == LT_SCORES ? br[x][y4] : br[y4][x]) = p0 * rb[q] - rn[q];
+            (KIND == LT_SCORES ? bs[x][y4] : bs[y4][x]) = rb[q];
+        }
+        __syncthreads();
+        k0 += 32;
+        if (k0 >= length(which)) which++, k0 = 0;
+        if (which < t.pairs) load(which, k0);
+#pragma unroll
+        for (int k = 0; k < 32; k += VEC<T>) {
+            Pack<T, VEC<T>> a[4], m[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                a[q] = *reinterpret_cast<const Pack<T, VEC<T>> *>(&as[y + 8 * q][k]);
+                m[q] = *reinterpret_cast<const Pack<T, VEC<T>> *>(&am[y + 8 * q][k]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC<T>; e++) {
+                const T r = br[k + e][x], b = bs[k + e][x];
+#pragma unroll
+                for (int q = 0; q < 4; q++) acc[q] += a[q].e[e] * r - m[q].e[e] * b;
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int row = t.i0 + y + 8 * q, col = t.j0 + x;
+        if (row >= t.rows || col >= t.cols || (KIND == LT_SCORES && col > row)) continue;
+        const int64_t o = t.at + (KIND == LT_SCORES ? int64_t(row) * (row + 1) / 2 : t.stride * row) + col;
+        out[o] = acc[q] + z[o];
+    }
+}
+
+// per chunk of a head: score_tiles tiles of the causal triangle, row by row, then the state's tiles
+template <typename T>
+__global__ void __launch_bounds__(LA_THREADS)
+    k_ls_chunk(const LaShape s, const __grid_constant__ LaChunkArgs<T> a, int score_tiles, int state_tiles)
+{
+    __shared__ alignas(16) T sm[4][32][LS_W<T>];
+    const int per = score_tiles + state_tiles, nc = s.chunks();
+    const int64_t r = blockIdx.x / per, bc = r / s.H, h = r - bc * s.H, b = bc / nc, bh = b * s.H + h;
+    const int which = int(blockIdx.x - r * per), c = int(bc - b * nc), len = s.len(c);
+    const int64_t row0 = (b * s.T + int64_t(c) * s.C) * a.ld, kd0 = int64_t(s.H) * s.dk;
+    LsTile<T> t;
+    LtPair<T> &p = t.p[0];
+    t.pairs = 1;
+    if (which < score_tiles) {
+        int i = 0;
+        while ((i + 1) * (i + 2) / 2 <= which) i++;
+        t.i0 = 32 * i, t.j0 = 32 * (which - i * (i + 1) / 2);
+        if (t.i0 >= len) return;
+        const int64_t oq = row0 + h * s.dk, ok = oq + kd0;
+        p.a = a.qkv + oq, p.a_ms = a.qkv_ms + oq, p.b = a.qkv + ok, p.b_ms = a.qkv_ms + ok;
+        p.lda = p.ldb = a.ld, p.K = s.dk, t.rows = t.cols = len;
+        t.at = bh * s.tri() + s.tri_at(c), t.stride = 0;
+        ls_tile<T, LT_SCORES>(sm, t, a.p0, a.qkv_ms != nullptr, a.z, a.out);
+    } else {
+        const int across = (s.dv + 31) / 32, i = (which - score_tiles) / across;
+        t.i0 = 32 * i, t.j0 = 32 * (which - score_tiles - i * across);
+        const int64_t ok = (bh * s.T + int64_t(c) * s.C) * s.dk, ov = row0 + 2 * kd0 + h * s.dv;
+        p.a = a.kd + ok, p.a_ms = a.kd_ms + ok, p.b = a.qkv + ov, p.b_ms = a.qkv_ms + ov;
+        p.lda = s.dk, p.ldb = a.ld, p.K = len, t.rows = s.dk, t.cols = s.dv;
+        t.at = s.n_scores() + (int64_t(c) * s.bh() + bh) * s.dk * s.dv, t.stride = s.dv;
+        ls_tile<T, LT_STATES>(sm, t, a.p0, a.qkv_ms != nullptr, a.z, a.out);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(LA_THREADS)
+    k_ls_output(const LaShape s, const __grid_constant__ LaOutArgs<T> a, int down, int across)
+{
+    __shared__ alignas(16) T sm[4][32][LS_W<T>];
+    const int per = down * across, nc = s.chunks();
+    const int64_t r = blockIdx.x / per, bc = r / s.H, h = r - bc * s.H, b = bc / nc, bh = b * s.H + h;
+    const int which = int(blockIdx.x - r * per), c = int(bc - b * nc), len = s.len(c);
+    LsTile<T> t;
+    LtPair<T> &p = t.p[0], &q = t.p[1];
+    t.i0 = 32 * (which / across), t.j0 = 32 * (which % across);
+    if (t.i0 >= len) return;
+    const int64_t t0 = b * s.T + int64_t(c) * s.C, ov = t0 * a.ld + 2 * int64_t(s.H) * s.dk + h * s.dv;
+    const int64_t op = bh * s.tri() + s.tri_at(c), oq = (bh * s.T + int64_t(c) * s.C) * s.dk;
+    const int64_t os = (c ? s.n_scores() + int64_t(c - 1) * s.n_state() : 0) + bh * s.dk * s.dv;
+    const T *const st = c ? a.ps : a.s0, *const st_ms = c ? a.ps_ms : a.s0_ms;
+    p.a = a.ps + op, p.a_ms = a.ps_ms + op, p.b = a.qkv + ov, p.b_ms = a.qkv_ms + ov, p.lda = 0, p.ldb = a.ld, p.K = len;
+    q.a = a.qd + oq, q.a_ms = a.qd_ms + oq, q.b = st + os, q.b_ms = st_ms + os, q.lda = s.dk, q.ldb = s.dv, q.K = s.dk;
+    t.pairs = st ? 2 : 1, t.rows = len, t.cols = s.dv;
+    t.at = (t0 * s.H + h) * s.dv, t.stride = int64_t(s.H) * s.dv;
+    ls_tile<T, LT_OUTPUT>(sm, t, a.p0, a.qkv_ms != nullptr, a.z, a.out);
+}
+
 // ------------------------------------------------------------------ one token
 //
 // A block takes CX x V columns of one head's state, its 256 / CX thread rows
@@ -797,10 +941,26 @@ static int la_tile_ready(K kern, uint32_t smem, int (&configured)[64], uint32_t 
 
 inline unsigned la_tile_grid(int64_t tiles) { return unsigned(tiles < 2 * 148 ? tiles : 2 * 148); }
 
+// The CUDA cores while their 32 x 32 tiles fit the SMs about at once, two rounds
+// at 32 bits, one at 64.  Chunk stage of 4 / 32 heads x 128 tokens x 64: 7.9 / 18.5
+// us there, 13.8 / 14.1 on the tensor cores; output stage 12.7 / 19.5 and 20.6 /
+// 21.0; over Z_2^64 chunk stage 15.1 / 39.6 and 24.9 / 34.6.
+template <typename T>
+static bool ls_fits(int64_t tiles)
+{
+    return tiles <= (sizeof(T) == 4 ? 2 * 148 : 148);
+}
+
 template <typename T>
 int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
 {
     if (!s.n_ps()) return DDG_OK;
+    const int rows = (s.len(0) + 31) / 32, tri = rows * (rows + 1) / 2;
+    const int square = ((s.dk + 31) / 32) * ((s.dv + 31) / 32);
+    if (ls_fits<T>(s.bh() * s.chunks() * (tri + square))) {
+        k_ls_chunk<T><<<unsigned(s.bh() * s.chunks() * (tri + square)), LA_THREADS, 0, st>>>(s, a, tri, square);
+        return launched();
+    }
     using S = LtShape<T>;
     static thread_local int configured[64];
     const int np = (s.len(0) + S::NT - 1) / S::NT, ns = (s.dv + S::NT - 1) / S::NT;
@@ -844,6 +1004,11 @@ template <typename T>
 int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
 {
     if (!s.n_out()) return DDG_OK;
+    const int down = (s.len(0) + 31) / 32, across = (s.dv + 31) / 32;
+    if (ls_fits<T>(s.bh() * s.chunks() * down * across)) {
+        k_ls_output<T><<<unsigned(s.bh() * s.chunks() * down * across), LA_THREADS, 0, st>>>(s, a, down, across);
+        return launched();
+    }
     using S = LtShape<T>;
     static thread_local int configured[64];
     const int tiles = (s.dv + S::NT - 1) / S::NT;
