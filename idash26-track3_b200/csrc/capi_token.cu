@@ -16,7 +16,7 @@ int check_q4(const ddg_q4_weights *w)
     DDG_CHECK(w->group > 0 && w->group % 32 == 0, DDG_ERR_ARG, "group must be a multiple of 32 (got %d)", w->group);
     DDG_CHECK(w->K == 0 || w->N == 0 || (w->d_q && w->d_step), DDG_ERR_ARG, "null pointer");
     DDG_CHECK((reinterpret_cast<uintptr_t>(w->d_q) & 15) == 0, DDG_ERR_ARG, "4-bit codes must be 16-byte aligned");
-    DDG_CHECK((reinterpret_cast<uintptr_t>(w->d_step) & 3) == 0, DDG_ERR_ARG, "4-bit steps must be 4-byte aligned");
+    DDG_CHECK((reinterpret_cast<uintptr_t>(w->d_step) & 1) == 0, DDG_ERR_ARG, "4-bit steps must be 2-byte aligned");
     return DDG_OK;
 }
 
@@ -31,7 +31,9 @@ int check_linattn(const ddg_linattn_shape *p, LaShape *s)
     s->B = p->batch, s->H = p->heads, s->T = p->tokens, s->dk = p->dk, s->dv = p->dv, s->C = p->chunk;
     s->pn = p->pow_n;
     const double tokens = double(p->tokens < 128 ? 128 : p->tokens);
-    DDG_CHECK(p->tokens <= (1 << 24), DDG_ERR_ARG, "%d tokens in one prompt (at most 2^24)", p->tokens);
+    // the carry's sums grow with the square of the chunks; a longer prompt goes on from the state
+    DDG_CHECK((int64_t(p->tokens) + p->chunk - 1) / p->chunk <= LA_MAX_CHUNKS, DDG_ERR_ARG,
+              "%d tokens are more than %d chunks of %d", p->tokens, LA_MAX_CHUNKS, p->chunk);
     DDG_CHECK(double(p->batch) * p->heads * tokens * 512.0 * 128.0 < 9e18 && double(p->heads) * 384.0 < 2e9,
               DDG_ERR_ARG, "linear attention sizes overflow");
     return DDG_OK;
@@ -57,9 +59,13 @@ int check_la(int bw, int party, const ddg_linattn_shape *p, int64_t ld, LaShape 
     return DDG_OK;
 }
 
-int check_ptrs(std::initializer_list<const void *> ptrs)
+// ring arrays: there, and on element boundaries
+int check_ptrs(int bw, std::initializer_list<const void *> ptrs)
 {
-    for (const void *p : ptrs) DDG_CHECK(p, DDG_ERR_ARG, "null pointer");
+    for (const void *p : ptrs) {
+        DDG_CHECK(p, DDG_ERR_ARG, "null pointer");
+        DDG_CHECK(reinterpret_cast<uintptr_t>(p) % uintptr_t(bw / 8) == 0, DDG_ERR_ARG, "misaligned ring array");
+    }
     return DDG_OK;
 }
 
@@ -133,7 +139,7 @@ int ddg_q4_quantize(int K, int N, int group, const int64_t *d_w, void *d_q, void
 {
     ddg_q4_weights w = {K, N, group, d_q, d_step, nullptr};
     DDG_TRY(check_q4(&w));
-    DDG_CHECK(K == 0 || N == 0 || d_w, DDG_ERR_ARG, "null pointer");
+    if (K && N) DDG_TRY(check_ptrs(64, {d_w}));
     return q4_quantize(K, N, group, d_w, static_cast<uint8_t *>(d_q), static_cast<uint16_t *>(d_step),
                        static_cast<cudaStream_t>(stream));
 }
@@ -147,14 +153,15 @@ int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const voi
     DDG_CHECK(ldx >= w->K, DDG_ERR_ARG, "row stride %lld below K = %d", (long long)ldx, w->K);
     const uint64_t n = uint64_t(M) * w->N;
     if (!n) return DDG_OK;
-    DDG_TRY(check_ptrs({d_c, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_c, d_out}));
     auto st = static_cast<cudaStream_t>(stream);
     if (party == 1) {
         if (d_out != d_c)
             DDG_CUDA(cudaMemcpyAsync(d_out, d_c, n * uint64_t(bw / 8), cudaMemcpyDeviceToDevice, st));
         return DDG_OK;
     }
-    DDG_CHECK(w->K == 0 || d_xhat, DDG_ERR_ARG, "null pointer");
+    if (w->K) DDG_TRY(check_ptrs(bw, {d_xhat}));
+    if (w->d_bias2s) DDG_TRY(check_ptrs(bw, {w->d_bias2s}));
     return bw == 32 ? fc_q4_t<uint32_t>(M, w, d_xhat, ldx, d_c, d_out, st)
                     : fc_q4_t<uint64_t>(M, w, d_xhat, ldx, d_c, d_out, st);
 }
@@ -197,7 +204,7 @@ int ddg_linattn_decay(int bw, const ddg_linattn_shape *shape, int64_t ld, const 
     LaShape s;
     DDG_TRY(check_la(bw, 0, shape, ld, &s));
     if (!s.n_qkv()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_pow, d_qkv, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_pow, d_qkv, d_out}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32 ? la_decay<uint32_t>(s, ld, in<uint32_t>(d_pow), in<uint32_t>(d_qkv),
                                          static_cast<uint32_t *>(d_out), st)
@@ -212,7 +219,7 @@ int ddg_linattn_carry(int bw, const ddg_linattn_shape *shape, const void *d_pow,
     DDG_TRY(check_ring(bw, 0));
     DDG_TRY(check_linattn(shape, &s));
     if (!s.n_ps()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_pow, d_ps, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_pow, d_ps, d_out, d_s0 ? d_s0 : d_ps}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32 ? la_carry<uint32_t>(s, in<uint32_t>(d_pow), in<uint32_t>(d_ps), in<uint32_t>(d_s0),
                                          static_cast<uint32_t *>(d_out), st)
@@ -227,7 +234,7 @@ int ddg_linattn_chunk_share(int bw, int party, const ddg_linattn_shape *shape, i
     LaShape s;
     DDG_TRY(check_la(bw, party, shape, ld, &s));
     if (!s.n_ps()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_qkv_hat, d_qkv_ms, d_kd_hat, d_kd_ms, d_z, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_qkv_hat, d_qkv_ms, d_kd_hat, d_kd_ms, d_z, d_out}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32 ? chunk_t<uint32_t>(party, s, ld, d_qkv_hat, d_qkv_ms, d_kd_hat, d_kd_ms, d_z, d_out, st)
                     : chunk_t<uint64_t>(party, s, ld, d_qkv_hat, d_qkv_ms, d_kd_hat, d_kd_ms, d_z, d_out, st);
@@ -242,7 +249,8 @@ int ddg_linattn_output_share(int bw, int party, const ddg_linattn_shape *shape, 
     DDG_TRY(check_la(bw, party, shape, ld, &s));
     DDG_CHECK(!d_s0_hat == !d_s0_ms, DDG_ERR_ARG, "the first state needs its value and its mask share");
     if (!s.n_out()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_qkv_hat, d_qkv_ms, d_qd_hat, d_qd_ms, d_ps_hat, d_ps_ms, d_z, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_qkv_hat, d_qkv_ms, d_qd_hat, d_qd_ms, d_ps_hat, d_ps_ms, d_z, d_out,
+                            d_s0_hat ? d_s0_hat : d_z, d_s0_ms ? d_s0_ms : d_z}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32 ? output_t<uint32_t>(party, s, ld, d_qkv_hat, d_qkv_ms, d_qd_hat, d_qd_ms, d_ps_hat, d_ps_ms,
                                          d_s0_hat, d_s0_ms, d_z, d_out, st)
@@ -258,7 +266,7 @@ int ddg_linattn_step_share(int bw, int party, const ddg_linattn_shape *shape, in
     DDG_TRY(check_la(bw, party, shape, ld, &s));
     DDG_CHECK(s.T == 1, DDG_ERR_ARG, "a step takes one token per sequence (got %d)", s.T);
     if (!s.bh()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_pow, d_qkv_hat, d_qkv_ms, d_s_hat, d_s_ms, d_z, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_pow, d_qkv_hat, d_qkv_ms, d_s_hat, d_s_ms, d_z, d_out}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32 ? step_t<uint32_t>(party, s, ld, d_pow, d_qkv_hat, d_qkv_ms, d_s_hat, d_s_ms, d_z, d_out, st)
                     : step_t<uint64_t>(party, s, ld, d_pow, d_qkv_hat, d_qkv_ms, d_s_hat, d_s_ms, d_z, d_out, st);
@@ -272,7 +280,7 @@ int ddg_linattn_step_output_share(int bw, int party, const ddg_linattn_shape *sh
     DDG_TRY(check_la(bw, party, shape, ld, &s));
     DDG_CHECK(s.T == 1, DDG_ERR_ARG, "a step takes one token per sequence (got %d)", s.T);
     if (!s.bh()) return DDG_OK;
-    DDG_TRY(check_ptrs({d_pow, d_qkv_hat, d_qkv_ms, d_yw_hat, d_yw_ms, d_z, d_out}));
+    DDG_TRY(check_ptrs(bw, {d_pow, d_qkv_hat, d_qkv_ms, d_yw_hat, d_yw_ms, d_z, d_out}));
     auto st = static_cast<cudaStream_t>(stream);
     return bw == 32
                ? step_output_t<uint32_t>(party, s, ld, d_pow, d_qkv_hat, d_qkv_ms, d_yw_hat, d_yw_ms, d_z, d_out, st)

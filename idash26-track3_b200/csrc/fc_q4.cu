@@ -482,7 +482,10 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         }
     } else if (tma_warp) {
         const bool leader = elect_one();
-        if (leader) tma_prefetch(&codes_map), tma_prefetch(&x_map);
+        if (leader) {
+            tma_prefetch(&codes_map);
+            if (vec) tma_prefetch(&x_map);
+        }
         for (int c = 0, r = 0; c < nk && ok; c++, r = r + 1 == S::RD ? 0 : r + 1) {
             // (not the full barriers: between two uses of a raw stage they can pass two phases, and a parity
             // tells only neighbouring ones apart)

@@ -35,7 +35,7 @@ inline int64_t la_blocks(int64_t n, int V) { return (n + int64_t(LA_THREADS) * V
 #define LA_EACH(e, n) \
     for (int64_t e = int64_t(blockIdx.x) * LA_THREADS + threadIdx.x; e < (n); e += int64_t(gridDim.x) * LA_THREADS)
 
-// chunk, row and column of entry e of one head's score triangles (e < 2^31: check_linattn)
+// chunk, row and column of entry e of one head's score triangles (e < 2^31: LA_MAX_CHUNKS)
 __device__ __forceinline__ void tri_find(const LaShape &s, int64_t e, int &c, int &i, int &j)
 {
     const uint32_t full = uint32_t(s.C) * uint32_t(s.C + 1) / 2;
@@ -806,9 +806,11 @@ __global__ void __launch_bounds__(LA_THREADS)
 // stride over dk: S, its mask share and the dealer's word are read once and
 // the new state written once (4 words moved and 5 multiply-adds per entry, so
 // bound by memory); q . S comes out of the same pass, summed over the thread
-// rows in shared memory.
+// rows in shared memory.  Two rows ahead and four blocks an SM: 1024 heads x 128 x
+// 128 in 50 us (5.3 TB/s), 512 x 64 x 128 over Z_2^64 in 31 us; four rows and three
+// blocks took 54 and 39, one wave of blocks that loop over heads 73 and 47.
 template <typename T, int V>
-__global__ void __launch_bounds__(LA_THREADS, 3)
+__global__ void __launch_bounds__(LA_THREADS, 4)
     k_la_step(const LaShape s, const __grid_constant__ LaStepArgs<T> a, int cx, int slabs)
 {
     __shared__ T qs[128], ks[128], rq[128], rk[128];
@@ -823,7 +825,7 @@ __global__ void __launch_bounds__(LA_THREADS, 3)
     const bool on = col < s.dv;
     // a thread's next U rows, in flight while the present ones are worked on (the
     // first ones while q, k and v arrive)
-    constexpr int U = 4;
+    constexpr int U = 2;
     PV S[U], m[U], z[U];
     const int64_t at = bh * per + col;
     auto fetch = [&](int i0) {

@@ -46,6 +46,7 @@ int q4_quantize(int K, int N, int group, const int64_t *w, uint8_t *q, uint16_t 
 //                     tri: per chunk the rows i = 0, 1, .. of its causal
 //                     triangle, i + 1 entries each
 // pow[h][n], n = 0..pn: lambda_h^n at the fixed-point scale.
+constexpr int LA_MAX_CHUNKS = 2048;  // chunks of one prompt call
 struct LaShape {
     int B = 0, H = 0, T = 0, dk = 0, dv = 0, C = 128, pn = 0;
     __host__ __device__ int64_t bh() const { return int64_t(B) * H; }

@@ -499,8 +499,8 @@ int ddg_op_output_keygen(ddg_dealer *dealer, ddg_cursor *cur, ddg_mask_wire *o);
  * d_q: output n's codes in one row of ddg_q4_row_bytes(K) bytes, code k in the
  * low half (k even) or the high half (k odd) of byte k/2; 16-byte aligned.
  * d_step: ceil(K / group) x N uint16 steps of 12 bits (higher bits are
- * ignored), so that every weight is below 2^15 in magnitude; 4-byte aligned.
- * group is a multiple of 32.  d_bias2s: N ring elements (bias << scale), or NULL. */
+ * ignored), so that every weight is below 2^15 in magnitude.  group is a
+ * multiple of 32.  d_bias2s: N ring elements (bias << scale), or NULL. */
 typedef struct ddg_q4_weights {
     int K, N, group;
     const void *d_q;
@@ -516,14 +516,16 @@ uint64_t ddg_q4_row_bytes(int K); /* 16 * ceil(K / 32); 0 for K < 1 */
 int ddg_q4_quantize(int K, int N, int group, const int64_t *d_w, void *d_q, void *d_step, void *stream);
 /* as ddg_fc_share with 4-bit weights, rows of x_hat ldx elements apart:
  *   party 0: out = x_hat . W + bias2s + C0;  party 1: out = C1
- * d_c and d_out (M x N) contiguous; d_out may be d_c. */
+ * d_c and d_out (M x N) contiguous; d_out may be d_c.  K is at most 262,144
+ * (a narrow accumulator's sums stay exact up to there). */
 int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const void *d_xhat, int64_t ldx,
                     const void *d_c, void *d_out, void *stream);
 
 /* Linear attention  S_t = lambda_h S_{t-1} + k_t v_t^T,  o_t = q_t S_t  (S is
  * dk x dv per head), for prompts in chunks of `chunk` tokens and for one token.
- * batch >= 0, heads >= 1, tokens in 0..2^24, dk, dv and chunk in 1..128;
- * pow_n >= tokens and >= 1.  Arrays, row-major, T = tokens, bh = batch * heads + head:
+ * batch >= 0, heads >= 1, tokens >= 0, dk, dv and chunk in 1..128, at most 2048
+ * chunks to a call (a longer prompt goes on from the state); pow_n >= tokens
+ * and >= 1.  Arrays, row-major, T = tokens, bh = batch * heads + head:
  *   qkv     (batch, T) rows, ld elements apart, each [q: heads x dk |
  *           k: heads x dk | v: heads x dv], ld >= heads * (2 dk + dv)
  *   pow     (heads, pow_n + 1): lambda_h^n at the scale (ddg_decay_table)
@@ -551,7 +553,8 @@ int ddg_decay_table(int bw, int scale, int heads, int n, const double *h_lambda,
 /* array sizes in ring elements: out6 = {qkv at the least ld, qkd, ps, state, step output, out} */
 int ddg_linattn_sizes(const ddg_linattn_shape *shape, int64_t *out6);
 /* the two public maps: on a masked value the masked result, on the dealer's
- * mask the result's mask (no key).  d_s0 may be NULL (a zero state). */
+ * mask the result's mask (no key).  d_s0 may be NULL (a zero state); d_out
+ * overlaps no input. */
 int ddg_linattn_decay(int bw, const ddg_linattn_shape *shape, int64_t ld, const void *d_pow, const void *d_qkv,
                       void *d_out, void *stream);
 int ddg_linattn_carry(int bw, const ddg_linattn_shape *shape, const void *d_pow, const void *d_ps, const void *d_s0,

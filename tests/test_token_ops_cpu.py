@@ -20,7 +20,7 @@ def la(ddg, batch=1, heads=2, tokens=5, dk=4, dv=3, chunk=4, pow_n=5):
 
 
 @pytest.mark.parametrize("kw", [dict(K=-1), dict(N=-1), dict(group=0), dict(group=48), dict(q=None), dict(step=None),
-                                dict(q=264), dict(step=258)])
+                                dict(q=264), dict(step=257)])
 def test_fc_q4_refuses_bad_weights(ddg, kw):
     assert ddg.lib().ddg_fc_q4_share(32, 0, 2, q4(ddg, **kw), 256, 64, 256, 256, None) == ARG
 
@@ -45,7 +45,7 @@ def test_fc_q4_null_weights_and_empty_calls(ddg):
 
 @pytest.mark.parametrize("kw", [dict(batch=-1), dict(heads=0), dict(tokens=-1), dict(dk=0), dict(dk=129), dict(dv=0),
                                 dict(dv=129), dict(chunk=0), dict(chunk=129), dict(pow_n=4),
-                                dict(tokens=0, pow_n=0), dict(tokens=(1 << 24) + 1, pow_n=1 << 25), dict(batch=1 << 30, heads=1 << 20, tokens=1 << 30,
+                                dict(tokens=0, pow_n=0), dict(tokens=8193, pow_n=8193), dict(tokens=2049, pow_n=2049, chunk=1), dict(batch=1 << 30, heads=1 << 20, tokens=1 << 30,
                                                               pow_n=1 << 30)])
 def test_linattn_refuses_bad_shapes(ddg, kw):
     L, s = ddg.lib(), la(ddg, **kw)
@@ -73,7 +73,6 @@ def test_linattn_refuses_bad_arguments(ddg):
     assert L.ddg_linattn_output_share(32, 0, s, w, *p[:6], 256, None, 256, 256, None) == ARG  # s0 without its mask share
     assert L.ddg_linattn_output_share(32, 0, s, w, *p[:6], None, 256, 256, 256, None) == ARG
     for fn in (L.ddg_linattn_step_share, L.ddg_linattn_step_output_share):
-        n = 7 if fn is L.ddg_linattn_step_share else 6
         n = len(fn.argtypes) - 5
         assert fn(32, 0, s, w, *p[:n], None) == ARG  # five tokens
         one = la(ddg, tokens=1)
@@ -89,6 +88,34 @@ def test_linattn_refuses_bad_arguments(ddg):
         assert L.ddg_linattn_output_share(64, 1, empty, w, *([None] * 10), None) == 0
         assert L.ddg_linattn_decay(64, empty, w, None, None, None, None) == 0
         assert L.ddg_linattn_carry(64, empty, None, None, None, None, None) == 0
+
+
+def test_misaligned_arrays_are_refused(ddg):
+    """A ring array off its element boundary would fault in a kernel: refused on the host, pointer by pointer."""
+    L, s, one, w = ddg.lib(), la(ddg), la(ddg, tokens=1), 22
+    for bw, off in ((32, 2), (64, 4)):
+        bad = 256 + off
+        for i in range(3):
+            a = [256, 256, 256]
+            a[i] = bad
+            assert L.ddg_fc_q4_share(bw, 0, 2, q4(ddg), a[0], 64, a[1], a[2], None) == ARG
+        assert L.ddg_fc_q4_share(bw, 0, 2, q4(ddg, b=bad), 256, 64, 256, 256, None) == ARG
+        calls = ((L.ddg_linattn_chunk_share, 6, s), (L.ddg_linattn_output_share, 10, s),
+                 (L.ddg_linattn_step_share, 7, one), (L.ddg_linattn_step_output_share, 7, one))
+        for fn, n, shape in calls:
+            for i in range(n):
+                a = [256] * n
+                a[i] = bad
+                assert fn(bw, 0, shape, w, *a, None) == ARG, (fn, i)
+        for i in range(3):
+            a = [256, 256, 256]
+            a[i] = bad
+            assert L.ddg_linattn_decay(bw, s, w, *a, None) == ARG
+        for i in range(4):
+            a = [256] * 4
+            a[i] = bad
+            assert L.ddg_linattn_carry(bw, s, *a, None) == ARG
+    assert L.ddg_q4_quantize(64, 8, 32, 260, 256, 256, None) == ARG
 
 
 def test_linattn_sizes(ddg):

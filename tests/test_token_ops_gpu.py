@@ -205,6 +205,83 @@ def test_linattn_step_shares(ddg, cuda, bw, party, B, H, dk, dv):
 
 
 @pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("BH,T", [(2, 40), (40, 256)])  # the CUDA-core tiles and the tensor cores
+def test_linattn_products_in_place_of_the_dealers_word(ddg, cuda, bw, BH, T):
+    """d_out may be d_z: every word is read before its place is written."""
+    rng = np.random.default_rng(BH + T + bw)
+    s, sh, ld, pow_ = la_inputs(ddg, rng, bw, (1, BH, T, 32, 48, 128))
+    x, rx, kd, rkd = (rnd(rng, bw, *n) for n in ((1, T, ld), (1, T, ld), (s.n_decayed,), (s.n_decayed,)))
+    ps, rps, z, z2 = (rnd(rng, bw, n) for n in (s.n_ps, s.n_ps, s.n_ps, T * BH * 48))
+    dx, drx, dkd, drkd, dps, drps, dz, dz2 = (to_dev(i) for i in (x, rx, kd, rkd, ps, rps, z, z2))
+    ddg.linattn_chunk_share(bw, 1, sh, ld, ptr(dx), ptr(drx), ptr(dkd), ptr(drkd), ptr(dz), ptr(dz))
+    ddg.linattn_output_share(bw, 0, sh, ld, ptr(dx), ptr(drx), ptr(dkd), ptr(drkd), ptr(dps), ptr(drps), None, None,
+                             ptr(dz2), ptr(dz2))
+    assert np.array_equal(from_dev(dz, z.dtype, z.size), R.ring(R.chunk_share(s, 1, x, rx, kd, rkd) + z, bw))
+    want = R.output_share(s, 0, x, rx, kd, rkd, ps, rps, None, None)
+    assert np.array_equal(from_dev(dz2, z.dtype, z2.size), R.ring(want + z2, bw))
+    s1, sh1, ld1, pow1 = la_inputs(ddg, rng, bw, (T, 2, 1, 64, 48, 128))
+    x, rx, st, rst = (rnd(rng, bw, *n) for n in ((T, 1, ld1), (T, 1, ld1), (s1.n_state,), (s1.n_state,)))
+    z = rnd(rng, bw, s1.n_state + T * 2 * 49)
+    dp, dx, drx, ds, drs, dz = (to_dev(i) for i in (pow1, x, rx, st, rst, z))
+    ddg.linattn_step_share(bw, 0, sh1, ld1, ptr(dp), ptr(dx), ptr(drx), ptr(ds), ptr(drs), ptr(dz), ptr(dz))
+    assert np.array_equal(from_dev(dz, z.dtype, z.size), R.ring(R.step_share(s1, 0, pow1[:, 1], x, rx, st, rst) + z, bw))
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("shape", [(1, 12, 520, 64, 64, 128), (1, 20, 300, 48, 96, 100), (1, 30, 200, 47, 33, 64),
+                                   (2, 16, 129, 32, 128, 128)])
+def test_linattn_many_heads(ddg, cuda, bw, shape):
+    """enough tiles for the tensor-core path, several per CTA: whole and ragged chunks, aligned and odd widths"""
+    rng = np.random.default_rng(sum(shape) + bw)
+    s, sh, ld, _ = la_inputs(ddg, rng, bw, shape)
+    x, rx = rnd(rng, bw, s.B, s.T, ld), rnd(rng, bw, s.B, s.T, ld)
+    kd, rkd, ps, rps = (rnd(rng, bw, n) for n in (s.n_decayed, s.n_decayed, s.n_ps, s.n_ps))
+    s0, rs0, z, z2 = (rnd(rng, bw, n) for n in (s.n_state, s.n_state, s.n_ps, s.B * s.T * s.H * s.dv))
+    d = [to_dev(i) for i in (x, rx, kd, rkd, ps, rps, s0, rs0, z, z2)]
+    for party in (0, 1):
+        out, read = guarded(s.n_ps, bw)
+        ddg.linattn_chunk_share(bw, party, sh, ld, *[ptr(i) for i in d[:4]], ptr(d[8]), ptr(out))
+        assert np.array_equal(read(), R.ring(R.chunk_share(s, party, x, rx, kd, rkd) + z, bw))
+        out, read = guarded(z2.size, bw)
+        ddg.linattn_output_share(bw, party, sh, ld, *[ptr(i) for i in d[:8]], ptr(d[9]), ptr(out))
+        assert np.array_equal(read(), R.ring(R.output_share(s, party, x, rx, kd, rkd, ps, rps, s0, rs0) + z2, bw))
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("M,K,N,group", [(600, 1100, 2000, 128), (1030, 130, 5000, 32), (260, 2050, 4100, 160),
+                                         (3, 40000, 260, 32), (20, 70000, 130, 64), (2, 5000, 4000, 96)])
+def test_fc_q4_large(ddg, cuda, bw, M, K, N, group):
+    """every tile, K split over clusters, two weight tiles per CTA, sums past one CTA's range, against float64 limbs"""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(M + K + N)
+    dt = torch.int32 if bw == 32 else torch.int64
+    rand = lambda *n: torch.randint(-(1 << (bw - 1)), (1 << (bw - 1)) - 1, n, dtype=dt, device="cuda", generator=g)  # noqa: E731
+    row = 16 * ((K + 31) // 32)
+    q = torch.randint(0, 256, (N, row), device="cuda", generator=g).to(torch.uint8)
+    st = torch.randint(0, 4096, ((K + group - 1) // group, N), device="cuda", generator=g).to(torch.int16)
+    x, C, b = rand(M, K), rand(M, N), rand(N)
+    out = torch.empty(M, N, dtype=dt, device="cuda")
+    torch.cuda.synchronize()
+    w = ddg.Q4Weights(K, N, group, ptr(q), ptr(st), ptr(b))
+    ddg.fc_q4_share(bw, 0, M, w, ptr(x), K, ptr(C), ptr(out))
+    code = torch.stack((q & 15, q >> 4), 2).reshape(N, -1)[:, :K].double() - 8
+    W = (code.t() * st.double().repeat_interleave(group, 0)[:K])
+    want = C.long() + b.long()
+    for i in range(bw // 16):  # 2^16 x 2^15 x K < 2^53: exact
+        want = want + (torch.matmul(((x.long() >> (16 * i)) & 0xFFFF).double(), W).long() << (16 * i))
+    assert torch.equal(out, want.to(dt))
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+def test_fc_q4_refuses_too_long_a_reduction(ddg, cuda):
+    d = dev_bytes(4096)
+    w = ddg.Q4Weights((1 << 18) + 1, 8, 32, ptr(d), ptr(d), None)
+    assert ddg.lib().ddg_fc_q4_share(32, 0, 4, w, ptr(d), (1 << 18) + 1, ptr(d), ptr(d), None) == 1
+
+
+@pytest.mark.parametrize("bw", [32, 64])
 def test_share_calls_on_a_stream_and_in_a_graph(ddg, cuda, bw):
     """The share calls run on the stream they are given and can be captured; a replay reads the inputs anew."""
     import torch
