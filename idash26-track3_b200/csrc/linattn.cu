@@ -201,11 +201,10 @@ __global__ void __launch_bounds__(LA_THREADS, 3)
 // Persistent kernels, two CTAs per SM over strided lists of tiles.  Eight warps
 // load the operands of the next K-step into registers (no detour through shared
 // memory, whose bandwidth the planes and the MMAs' own reads take), split the
-// present one into planes and hand a stage to the MMA warp by mbarrier; there is
-// no CTA-wide barrier in the loop, and loads run on across tiles.  What bounds
-// these kernels is the latency of that chain in each warp (2000 cycles a step
-// with one CTA per SM), then the loads' lines in flight, so there are two CTAs,
-// every load covers whole 128-byte lines, and whole tiles take loads without
+// present one into planes and hand the stage over by mbarrier; there is no
+// CTA-wide barrier in the loop, and loads run on across tiles.  What bounds
+// these kernels is the loads' latency against what the registers hold in flight,
+// so every load covers whole 128-byte lines and whole tiles take loads without
 // bounds.
 constexpr int LT_WARPS = 8, LT_THREADS = LT_WARPS * 32;
 
@@ -310,28 +309,25 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
     // arrivals and barriers without waiting or writing, and the launch reports it.
     bool ok = true;
 
-    if (warp == LT_WARPS) {
+    {
+        // Warp 0 also issues the MMAs, a step's at the start of the next one, when the other warps' planes are
+        // likely there (a warp of its own for them would leave 96 registers a thread instead of 128).
         const bool leader = elect_one();
-        uint32_t g = 0;  // K-steps so far
-        for (int64_t t = first; t < tiles; t += step) {
-            const int steps = tile_of(t).steps;
-            for (int s = 0; s < steps; s++, g++) {
-                const uint32_t st = g % NST;
-                if (ok) ok = mbar_wait(&full[st], (g / NST) & 1);
-                tc_fence_after();
-                if (ok && leader) {
-                    const uint32_t sa = smem_addr(smem + st * S::STAGE);
-                    const uint64_t da = smem_desc(sa, 128, S::SBO), db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
+        auto multiply = [&](uint32_t g, bool first) {
+            const uint32_t st = g % NST;
+            if (ok) ok = mbar_wait(&full[st], (g / NST) & 1);
+            tc_fence_after();
+            if (ok && leader) {
+                const uint32_t sa = smem_addr(smem + st * S::STAGE);
+                const uint64_t da = smem_desc(sa, 128, S::SBO), db = smem_desc(sa + P * S::A_PLANE, 128, S::SBO);
 #pragma unroll
-                    for (int i = 0; i < P; i++)  // the address field counts 16-byte units
-                        mma_i8(tmem + uint32_t(i * NT), da + uint64_t(i * S::A_PLANE >> 4), db, i8_idesc((P - i) * NT, false),
-                               (s > 0 || i > 0) ? 1u : 0u);
-                    mma_commit(&empty[st]);
-                }
-                __syncwarp();
+                for (int i = 0; i < P; i++)  // the address field counts 16-byte units
+                    mma_i8(tmem + uint32_t(i * NT), da + uint64_t(i * S::A_PLANE >> 4), db, i8_idesc((P - i) * NT, false),
+                           (!first || i > 0) ? 1u : 0u);
+                mma_commit(&empty[st]);
             }
-        }
-    } else {
+            __syncwarp();
+        };
         // This thread's items of a K-step.  Rows of k: A rows krow + 32 j, B rows (columns of the tile)
         // brow + 32 j, four k from 4 kq.  k-major: 4 x 4 blocks of rows trow.. and k 4 tkq.. .
         constexpr bool A_T = KIND == LT_STATES, B_T = KIND != LT_SCORES;
@@ -531,6 +527,7 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
         load_next();
         while (ci < tiles) {
             const uint32_t st = g % NST;
+            if (warp == 0 && cs > 0) multiply(g - 1, cs == 1);
             if (g >= NST && ok) ok = mbar_wait(&empty[st], (g / NST - 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) split(r, st);
@@ -540,6 +537,7 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
             if (lane == 0) mbar_arrive(&full[st]);
             g++;
             if (++cs == slot(n).steps) {
+                if (warp == 0) multiply(g - 1, cs == 1);
                 epilogue(slot(n), g - 1);
                 n++, cs = 0, ci += step;
             }
@@ -558,7 +556,7 @@ inline __host__ __device__ int steps32(int k) { return (k + 31) / 32; }
 
 // CTAs below score_ctas take score tiles (columns 0, NT, .. of each chunk), the others state tiles
 template <typename T>
-__global__ void __launch_bounds__(LT_THREADS + 32, 2)
+__global__ void __launch_bounds__(LT_THREADS, 2)
     k_la_chunk(const LaShape s, const __grid_constant__ LaChunkArgs<T> a, int score_tiles, int state_tiles, int score_ctas,
                uint32_t *err)
 {
@@ -623,7 +621,7 @@ __global__ void __launch_bounds__(LT_THREADS + 32, 2)
 
 // tiles of chunk c of head bh: output columns 0, NT, ..
 template <typename T>
-__global__ void __launch_bounds__(LT_THREADS + 32, 2)
+__global__ void __launch_bounds__(LT_THREADS, 2)
     k_la_output(const LaShape s, const __grid_constant__ LaOutArgs<T> a, int64_t count, int tiles, uint32_t *err)
 {
     constexpr int NT = LtShape<T>::NT;
@@ -974,7 +972,7 @@ int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
     const double cs = double(scores) * (2 * steps32(s.dk) + 3), ct = double(states) * (2 * steps32(s.len(0)) + 3);
     int64_t mine = int64_t(double(grid) * cs / (cs + ct) + 0.5);
     mine = mine < 1 ? 1 : mine > grid - 1 ? grid - 1 : mine;
-    k_la_chunk<T><<<unsigned(grid), LT_THREADS + 32, S::SMEM, st>>>(s, a, np, ns, int(mine), err);
+    k_la_chunk<T><<<unsigned(grid), LT_THREADS, S::SMEM, st>>>(s, a, np, ns, int(mine), err);
     return launched();
 }
 
@@ -1017,7 +1015,7 @@ int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
     const int64_t count = s.bh() * s.chunks() * tiles;
     uint32_t *err = nullptr;
     DDG_TRY(la_tile_ready(k_la_output<T>, S::SMEM, configured, &err));
-    k_la_output<T><<<la_tile_grid(count), LT_THREADS + 32, S::SMEM, st>>>(s, a, count, tiles, err);
+    k_la_output<T><<<la_tile_grid(count), LT_THREADS, S::SMEM, st>>>(s, a, count, tiles, err);
     return launched();
 }
 
