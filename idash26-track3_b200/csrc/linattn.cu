@@ -341,15 +341,16 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
         struct Regs {
             T a[4][4], b[BI][4], m[BI][4];
             bool neg;
+            int skip;  // scores: rows above the tile's first column have no entry in it, their items stay out
         };
 
         auto load = [&](const LtTile<T> &t, int s, Regs &r) {
             const bool second = KIND == LT_OUTPUT && s >= t.steps0;
             const LtPair<T> &p = t.p[second ? 1 : 0];
             const int i = second ? s - t.steps0 : s;
+            r.skip = KIND == LT_SCORES ? t.j0 >> 5 : 0;
             r.neg = beaver && (i & 1);
             const int k0 = (beaver ? i >> 1 : i) * 32;
-            const bool with_m = beaver && !r.neg;
             const T *const a = r.neg ? p.a_ms : p.a;
             const int64_t lda = p.lda, ldb = p.ldb;
             if constexpr (A_T) {
@@ -372,21 +373,23 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
                 const T *q = a + krow * lda + k0 + 4 * kq;
                 if (p.whole_a) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++, q += 32 * lda) load4<T>(q, r.a[j]);
+                    for (int j = 0; j < 4; j++, q += 32 * lda)
+                        if (j >= r.skip) load4<T>(q, r.a[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; j++, q += 32 * lda)
-                        load4<T>(q, krow + 32 * j < t.rows ? p.K - k0 - 4 * kq : 0, p.vec_a, r.a[j]);
+                        if (j >= r.skip) load4<T>(q, krow + 32 * j < t.rows ? p.K - k0 - 4 * kq : 0, p.vec_a, r.a[j]);
                 }
             }
-            if (!b_on) return;
+            // the second step of a pair takes the B of the first, still in its registers
+            if (!b_on || r.neg) return;
             if constexpr (B_ONE) {
                 const int64_t o = int64_t(k0 + 4 * tkq) * ldb + bcol;
                 const int n = p.whole_b ? 4 : bcol < t.cols ? p.K - k0 - 4 * tkq : 0;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     r.b[0][e] = e < n ? __ldg(p.b + o + e * ldb) : T(0);
-                    if (with_m) r.m[0][e] = e < n ? __ldg(p.b_ms + o + e * ldb) : T(0);
+                    r.m[0][e] = beaver && e < n ? __ldg(p.b_ms + o + e * ldb) : T(0);
                 }
                 return;
             }
@@ -396,7 +399,7 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
             if (p.whole_b) {
 #pragma unroll
                 for (int e = 0; e < BI; e++, q += inc) load4<T>(q, r.b[e]);
-                if (with_m) {
+                if (beaver) {
 #pragma unroll
                     for (int e = 0; e < BI; e++, m += inc) load4<T>(m, r.m[e]);
                 }
@@ -406,7 +409,7 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
                     const int n = B_T ? (k0 + 4 * tkq + e < p.K ? t.cols - trow : 0)
                                       : (krow + 32 * e < t.cols ? p.K - k0 - 4 * kq : 0);
                     load4<T>(q, n, p.vec_b, r.b[e]);
-                    if (with_m) load4<T>(m, n, p.vec_b, r.m[e]);
+                    if (beaver) load4<T>(m, n, p.vec_b, r.m[e]);
                 }
             }
         };
@@ -421,27 +424,24 @@ __device__ __forceinline__ void la_tiles(int64_t first, int64_t step, int64_t ti
             for (int j = 0; j < 4; j++) {
                 const T e[4] = {A_T ? r.a[0][j] : r.a[j][0], A_T ? r.a[1][j] : r.a[j][1], A_T ? r.a[2][j] : r.a[j][2],
                                 A_T ? r.a[3][j] : r.a[j][3]};
-                store_planes<T>(pa, S::A_PLANE, j * a_inc, e);
+                if (j >= r.skip) store_planes<T>(pa, S::A_PLANE, j * a_inc, e);
             }
             if (!b_on) return;
-            if (r.neg) {
+            auto planes = [&](auto &&right) {
 #pragma unroll
-                for (int i = 0; i < BI; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) r.b[i][e] = T(0) - r.b[i][e];
-            } else if (beaver) {
-#pragma unroll
-                for (int i = 0; i < BI; i++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) r.b[i][e] = p0 * r.b[i][e] - r.m[i][e];
-            }
-#pragma unroll
-            for (int j = 0; j < BI; j++) {
-                constexpr bool X = B_T && !B_ONE;
-                const T e[4] = {X ? r.b[0][j] : r.b[j][0], X ? r.b[1 % BI][j] : r.b[j][1], X ? r.b[2 % BI][j] : r.b[j][2],
-                                X ? r.b[3 % BI][j] : r.b[j][3]};
-                store_planes<T>(pb, S::B_PLANE, j * b_inc, e);
-            }
+                for (int j = 0; j < BI; j++) {
+                    constexpr bool X = B_T && !B_ONE;
+                    const T e[4] = {X ? right(0, j) : right(j, 0), X ? right(1 % BI, j) : right(j, 1),
+                                    X ? right(2 % BI, j) : right(j, 2), X ? right(3 % BI, j) : right(j, 3)};
+                    store_planes<T>(pb, S::B_PLANE, j * b_inc, e);
+                }
+            };
+            if (r.neg)
+                planes([&](int i, int e) { return T(0) - r.b[i][e]; });
+            else if (beaver)
+                planes([&](int i, int e) { return p0 * r.b[i][e] - r.m[i][e]; });
+            else
+                planes([&](int i, int e) { return r.b[i][e]; });
         };
 
         T *const tile = reinterpret_cast<T *>(smem);
