@@ -14,6 +14,10 @@
 //   C = sum_s 2^(8s) sum_{i+j=s} A_i . B_j  (u8 x u8 -> s32, exact: K <= 512)
 // in tensor memory.  The limbs of B are stacked along N, so one MMA per limb i
 // of A covers every j with i + j < P, landing in the columns of s = i .. P-1.
+//
+// Measured on one B200 for 4 x 16 heads x 2048 tokens x 64 x 64 over Z_2^32 (ncu):
+// decay 29 us (4.6 TB/s), chunk stage 131 us (2.8 TB/s of 369 MB), carry 28 us
+// (3.6 TB/s), output stage 85 us (3.6 TB/s of 302 MB).
 #include "token.cuh"
 #include "umma.cuh"
 
@@ -941,14 +945,16 @@ static int la_tile_ready(K kern, uint32_t smem, int (&configured)[64], uint32_t 
 
 inline unsigned la_tile_grid(int64_t tiles) { return unsigned(tiles < 2 * 148 ? tiles : 2 * 148); }
 
-// The CUDA cores while their 32 x 32 tiles fit the SMs about at once, two rounds
-// at 32 bits, one at 64.  Chunk stage of 4 / 32 heads x 128 tokens x 64: 7.9 / 18.5
-// us there, 13.8 / 14.1 on the tensor cores; output stage 12.7 / 19.5 and 20.6 /
-// 21.0; over Z_2^64 chunk stage 15.1 / 39.6 and 24.9 / 34.6.
-template <typename T>
-static bool ls_fits(int64_t tiles)
+// The CUDA cores while their 32 x 32 tiles (a short last chunk has fewer) take
+// one round on the SMs, or two for the chunk stage at 32 bits.  For 4 / 16 / 32
+// heads x 128 tokens x 64, in us on CUDA cores against tensor cores: chunk stage
+// 8.0 / 12.8 / 18.4 against 14.5 / 14.8 / 15.1, over Z_2^64 15.2 / 27.1 / 39.6
+// against 22.0 / 22.4 / 27.0; output stage 12.7 / 13.0 / 19.5 against 17.1 / 17.3 /
+// 17.4, over Z_2^64 23.7 / 24.1 / 41.6 against 23.0 / 23.3 / 23.4, and for 16 heads
+// x 32 tokens there 13.0 against 14.0.
+static bool ls_fits(const LaShape &s, int64_t tiles_full, int64_t tiles_last, int rounds)
 {
-    return tiles <= (sizeof(T) == 4 ? 2 * 148 : 148);
+    return s.bh() * ((s.chunks() - 1) * tiles_full + tiles_last) <= rounds * 148;
 }
 
 template <typename T>
@@ -957,7 +963,8 @@ int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
     if (!s.n_ps()) return DDG_OK;
     const int rows = (s.len(0) + 31) / 32, tri = rows * (rows + 1) / 2;
     const int square = ((s.dk + 31) / 32) * ((s.dv + 31) / 32);
-    if (ls_fits<T>(s.bh() * s.chunks() * (tri + square))) {
+    const int last = (s.len(s.chunks() - 1) + 31) / 32;
+    if (ls_fits(s, tri + square, last * (last + 1) / 2 + square, sizeof(T) == 4 ? 2 : 1)) {
         k_ls_chunk<T><<<unsigned(s.bh() * s.chunks() * (tri + square)), LA_THREADS, 0, st>>>(s, a, tri, square);
         return launched();
     }
@@ -1005,7 +1012,7 @@ int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
 {
     if (!s.n_out()) return DDG_OK;
     const int down = (s.len(0) + 31) / 32, across = (s.dv + 31) / 32;
-    if (ls_fits<T>(s.bh() * s.chunks() * down * across)) {
+    if (ls_fits(s, down * across, (s.len(s.chunks() - 1) + 31) / 32 * across, 1)) {
         k_ls_output<T><<<unsigned(s.bh() * s.chunks() * down * across), LA_THREADS, 0, st>>>(s, a, down, across);
         return launched();
     }
