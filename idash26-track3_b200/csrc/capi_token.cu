@@ -20,6 +20,16 @@ int check_q4(const ddg_q4_weights *w)
     return DDG_OK;
 }
 
+// the same answer on the dealer and both parties, although party 1 multiplies nothing
+int check_q4_call(const ddg_q4_weights *w, int bw, int M)
+{
+    DDG_TRY(check_q4(w));
+    DDG_CHECK(M >= 0, DDG_ERR_ARG, "negative size");
+    DDG_CHECK(w->K <= Q4_MAX_K, DDG_ERR_ARG, "K = %d is too long (at most %d)", w->K, Q4_MAX_K);
+    DDG_CHECK(M <= q4_max_rows(bw), DDG_ERR_ARG, "%d rows are too many for one call (at most %d)", M, q4_max_rows(bw));
+    return DDG_OK;
+}
+
 int check_linattn(const ddg_linattn_shape *p, LaShape *s)
 {
     DDG_CHECK(p, DDG_ERR_ARG, "null linear attention shape");
@@ -148,8 +158,7 @@ int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const voi
                     const void *d_c, void *d_out, void *stream)
 {
     DDG_TRY(check_ring(bw, party));
-    DDG_TRY(check_q4(w));
-    DDG_CHECK(M >= 0, DDG_ERR_ARG, "negative size");
+    DDG_TRY(check_q4_call(w, bw, M));
     DDG_CHECK(ldx >= w->K, DDG_ERR_ARG, "row stride %lld below K = %d", (long long)ldx, w->K);
     const uint64_t n = uint64_t(M) * w->N;
     if (!n) return DDG_OK;

@@ -23,6 +23,12 @@
 // weights take P(P+1)/2.  One warp loads codes and x with TMA, one issues the
 // MMAs, the others expand codes and split x.  The sums of a split K meet in the
 // cluster's shared memory.
+//
+// Measured on one B200 (graph replays, launch included): CUDA cores, 1 x 376 x
+// 1024 4.3 us and 1 x 2048 x 4096 5.4 us; tensor cores, 256 x 1024 x 512 7.1 us,
+// 16 x 4096 x 8192 15.0 us (16.8 MB of codes, 1.1 TB/s: bound by the expansion
+// in its sixteen warps), 2048 x 4096 x 4096 230 us (0.30 P ring flop/s, 1.2 P byte
+// products/s: tensor pipe 62 % busy, bound by shared memory).
 #include <type_traits>
 
 #include "tma.cuh"
@@ -217,7 +223,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
 
 // ------------------------------------------------------------------ more rows: tensor cores
 
-constexpr int QT_MAX_K = 32768;            // k per CTA: a column's sum, 2 * 255^2 * K, stays below 2^32
+constexpr int QT_MAX_K = Q4_MAX_K / 8;     // k per CTA: a column's sum, 2 * 255^2 * K, stays below 2^32
 // operands lie in 16-byte chunks of 8 k, chunk-major: rows 16 bytes apart,
 // chunks of A 2048 and of B 16 NB + 16 bytes apart (the pad spreads the chunks
 // of one row, written by neighbouring lanes, over the banks)
@@ -763,14 +769,14 @@ int fc_q4(const Q4Args<T> &a, cudaStream_t st)
     }
     const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
     // the CUDA cores for one or two rows while the product is small: 1 x 1024 x 1024 takes 4.4 us there and
-    // 5.6 on the tensor cores, 1 x 4096 x 4096 over Z_2^64 13.8 and 10.7
+    // 5.5 on the tensor cores, 1 x 4096 x 4096 over Z_2^64 13.2 and 10.7
     const uint64_t macs = uint64_t(a.M) * uint64_t(a.w.K) * uint64_t(a.w.N);
     if (a.M <= 2 && macs * sizeof(T) <= (1u << 25) && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
         return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
     // The tile of least estimated time.  Wide tiles expand the weights fewer times
     // and split x for more outputs, narrow ones spread a small product over more
-    // SMs: 256 x 1024 x 512 takes 7.9 us in tiles of 16 rows and 9.8 in tiles of
-    // 64; 256 x 4096 x 8192 takes 103 us in tiles of 64 rows by 128 outputs and 59
+    // SMs: 256 x 1024 x 512 takes 7.1 us in tiles of 32 rows and 9.0 in tiles of
+    // 64; 256 x 4096 x 8192 takes 92 us in tiles of 64 rows by 128 outputs and 58
     // by 256.  Stage times (us per 64 k) are fits to such measurements.
     constexpr int F = sizeof(T) / 4;
     struct Tile {

@@ -188,7 +188,7 @@ int check_floor(int bw, int s)
 
 int check_fc_q4(const ddg_q4_weights *w, int bw, int s, int rows, int act)
 {
-    DDG_TRY(check_q4(w));
+    DDG_TRY(check_q4_call(w, bw, rows));
     DDG_CHECK(w->K > 0 && w->N > 0 && rows > 0, DDG_ERR_ARG, "bad FC sizes (%d rows, %d x %d)", rows, w->K, w->N);
     DDG_CHECK(act_ok(act) || act == FC_ACT_FLOOR, DDG_ERR_ARG, "act %d out of range", act);
     if (act == FC_ACT_FLOOR) return check_floor(bw, s);

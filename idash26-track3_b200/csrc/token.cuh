@@ -19,6 +19,9 @@ struct Q4 {
 };
 inline uint64_t q4_row_bytes(int K) { return 16ull * ((uint64_t(K) + 31) / 32); }
 constexpr int Q4_STEP_MAX = 4095;
+// what one call covers: a cluster of eight CTAs along K, grid rows of 64 (32 over Z_2^64) rows of x
+constexpr int Q4_MAX_K = 8 * 32768;
+constexpr int q4_max_rows(int bw) { return 65535 * (2048 / bw); }
 
 // out[m][n] = sign * (x . W)[m][n] + bias[n] + Add[m][n] (bias, Add may be null)
 template <typename T>
@@ -129,6 +132,7 @@ int la_step_output(const LaShape &s, const LaStepOutArgs<T> &a, cudaStream_t st)
 
 // argument checks of the C ABI's structs (capi_token.cu)
 int check_q4(const ddg_q4_weights *w);
+int check_q4_call(const ddg_q4_weights *w, int bw, int M);
 int check_linattn(const ddg_linattn_shape *p, LaShape *s);
 
 }  // namespace ddg

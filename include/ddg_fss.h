@@ -517,7 +517,8 @@ int ddg_q4_quantize(int K, int N, int group, const int64_t *d_w, void *d_q, void
 /* as ddg_fc_share with 4-bit weights, rows of x_hat ldx elements apart:
  *   party 0: out = x_hat . W + bias2s + C0;  party 1: out = C1
  * d_c and d_out (M x N) contiguous; d_out may be d_c.  K is at most 262,144
- * (a narrow accumulator's sums stay exact up to there). */
+ * (the accumulators' sums stay exact up to there) and M at most 4,194,240 over
+ * Z_2^32, 2,097,120 over Z_2^64. */
 int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const void *d_xhat, int64_t ldx,
                     const void *d_c, void *d_out, void *stream);
 
@@ -582,7 +583,7 @@ int ddg_linattn_step_output_share(int bw, int party, const ddg_linattn_shape *sh
  * are exact for values in [-2^(bw-2), 2^(bw-2)): the dealer shifts the masks
  * of the non-negative truncation gate by 2^(bw-2).  2 <= scale < bw - 2.
  * act: DDG_ACT_NONE, DDG_ACT_RELU, DDG_ACT_TRUNC as in ddg_op_fc_*, or
- * DDG_ACT_FLOOR, the floor just described (a tenth of DDG_ACT_TRUNC's key
+ * DDG_ACT_FLOOR, the floor just described (less than a tenth of DDG_ACT_TRUNC's key
  * bytes).  d_pow and the members of w are device arrays, the same on the
  * dealer and both parties.  Prompts and steps take the state as a wire and
  * give it back as one; a prompt's s0 may be NULL.  The key-byte functions count

@@ -191,3 +191,13 @@ def test_restatement_follows_the_recurrence(ddg):
     assert np.max(np.abs(np.stack(steps, 2) - np.stack(want, 2))) < tol
     for got in (S, Si):
         assert np.max(np.abs(got.view(np.int64).reshape(Sf.shape) / 2**scale - Sf)) < tol
+
+
+@pytest.mark.parametrize("party", [0, 1])
+@pytest.mark.parametrize("bw,M,K", [(32, 2, (1 << 18) + 1), (64, 2, (1 << 18) + 1), (32, 65535 * 64 + 1, 64),
+                                    (64, 65535 * 32 + 1, 64)])
+def test_fc_q4_overlong_calls_are_refused_alike(ddg, party, bw, M, K):
+    # party 1 multiplies nothing, but has to give its peer's answer
+    L = ddg.lib()
+    assert L.ddg_fc_q4_share(bw, party, M, q4(ddg, K=K), 256, K, 256, 256, None) == ARG
+    assert L.ddg_op_fc_q4_key_bytes(bw, 12, K, 8, M, ddg.ACT_NONE) == 0
