@@ -662,7 +662,11 @@ __global__ void __launch_bounds__(LT_THREADS, 2)
 //
 // The same products on the CUDA cores, in 32 x 32 tiles, for calls whose few
 // 128-row tiles would leave most SMs idle and run at one tile's latency.  256
-// threads, four rows of one column each; the next 32 k on their way in registers.
+// threads load 32 k at a time, the next ones on their way in registers; four
+// groups of 64 threads take 8 k each, 4 x 4 entries a thread, and their sums meet
+// in shared memory.  (4 x 1 entries a thread, all k, read shared memory more often
+// than they multiplied: the chunk stage of 8 heads x 128 tokens x 64 took 7.9 us
+// instead of 7.0.)
 template <typename T>
 struct LsTile {
     LtPair<T> p[2];
@@ -671,17 +675,19 @@ struct LsTile {
 };
 
 template <typename T>
-constexpr int LS_W = 32 + VEC<T>;  // row pitch: 16-byte rows for the A reads, off the banks of the next row
+constexpr int LS_W = 32 + VEC<T>;  // row pitch: 16-byte reads, off the banks of the next row
 template <typename T, int KIND>
 __device__ __forceinline__ void ls_tile(T (&sm)[4][32][LS_W<T>], const LsTile<T> &t, T p0, bool beaver, const T *z, T *out)
 {
-    // A, [A] (row, k); p0 B - [B], B (k, column)
+    // A, -[A] (k, row); p0 B - [B], B (k, column)
     auto &as = sm[0], &am = sm[1], &br = sm[2], &bs = sm[3];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    T acc[4] = {0, 0, 0, 0};
+    const int group = threadIdx.x >> 6, ty = 4 * ((threadIdx.x & 63) >> 3), tx = 4 * (threadIdx.x & 7);
+    T acc[4][4] = {};
     T ra[4], rm[4], rb[4], rn[4];
     auto load = [&](int which, int k0) {
-        const LtPair<T> &p = t.p[which];
+        LtPair<T> p = t.p[0];  // (indexed by `which` it would lie in local memory)
+        if (KIND == LT_OUTPUT && which) p = t.p[1];
         const bool tri = KIND == LT_OUTPUT && which == 0;
 #pragma unroll
         for (int q = 0; q < 4; q++) {
@@ -702,8 +708,8 @@ __device__ __forceinline__ void ls_tile(T (&sm)[4][32][LS_W<T>], const LsTile<T>
     };
     // entries right of a causal tile's last row add nothing
     auto length = [&](int which) {
-        const int K = t.p[which].K;
-        return KIND == LT_OUTPUT && which == 0 && t.i0 + 32 < K ? t.i0 + 32 : K;
+        if (KIND != LT_OUTPUT) return t.p[0].K;
+        return which ? t.p[1].K : t.i0 + 32 < t.p[0].K ? t.i0 + 32 : t.p[0].K;
     };
     int which = 0, k0 = 0;
     load(0, 0);
@@ -712,7 +718,7 @@ __device__ __forceinline__ void ls_tile(T (&sm)[4][32][LS_W<T>], const LsTile<T>
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const int y4 = y + 8 * q;
-            (KIND == LT_STATES ? as[x][y4] : as[y4][x]) = ra[q], (KIND == LT_STATES ? am[x][y4] : am[y4][x]) = rm[q];
+            (KIND == LT_STATES ? as[y4][x] : as[x][y4]) = ra[q], (KIND == LT_STATES ? am[y4][x] : am[x][y4]) = T(0) - rm[q];
             (KIND == LT_SCORES ? br[x][y4] : br[y4][x]) = p0 * rb[q] - rn[q];
             (KIND == LT_SCORES ? bs[x][y4] : bs[y4][x]) = rb[q];
         }
@@ -720,28 +726,42 @@ __device__ __forceinline__ void ls_tile(T (&sm)[4][32][LS_W<T>], const LsTile<T>
         k0 += 32;
         if (k0 >= length(which)) which++, k0 = 0;
         if (which < t.pairs) load(which, k0);
+        auto four = [](const T *p, T (&e)[4]) {
 #pragma unroll
-        for (int k = 0; k < 32; k += VEC<T>) {
-            Pack<T, VEC<T>> a[4], m[4];
+            for (int i = 0; i < 4; i += VEC<T>) {
+                const Pack<T, VEC<T>> v = *reinterpret_cast<const Pack<T, VEC<T>> *>(p + i);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                a[q] = *reinterpret_cast<const Pack<T, VEC<T>> *>(&as[y + 8 * q][k]);
-                m[q] = *reinterpret_cast<const Pack<T, VEC<T>> *>(&am[y + 8 * q][k]);
+                for (int j = 0; j < VEC<T>; j++) e[i + j] = v.e[j];
             }
+        };
 #pragma unroll
-            for (int e = 0; e < VEC<T>; e++) {
-                const T r = br[k + e][x], b = bs[k + e][x];
+        for (int k = 8 * group, n = 0; n < 8; n++, k++) {
+            T a[4], m[4], r[4], b[4];
+            four(&as[k][ty], a), four(&am[k][ty], m), four(&br[k][tx], r), four(&bs[k][tx], b);
 #pragma unroll
-                for (int q = 0; q < 4; q++) acc[q] += a[q].e[e] * r - m[q].e[e] * b;
-            }
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[i][j] += a[i] * r[j] + m[i] * b[j];
         }
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j += VEC<T>) {
+            Pack<T, VEC<T>> v;
+#pragma unroll
+            for (int e = 0; e < VEC<T>; e++) v.e[e] = acc[i][j + e];
+            *reinterpret_cast<Pack<T, VEC<T>> *>(&sm[group][ty + i][tx + j]) = v;
+        }
+    __syncthreads();
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         const int row = t.i0 + y + 8 * q, col = t.j0 + x;
         if (row >= t.rows || col >= t.cols || (KIND == LT_SCORES && col > row)) continue;
         const int64_t o = t.at + (KIND == LT_SCORES ? int64_t(row) * (row + 1) / 2 : t.stride * row) + col;
-        out[o] = acc[q] + z[o];
+        const int a = y + 8 * q;
+        out[o] = sm[0][a][x] + sm[1][a][x] + sm[2][a][x] + sm[3][a][x] + z[o];
     }
 }
 
@@ -946,15 +966,16 @@ static int la_tile_ready(K kern, uint32_t smem, int (&configured)[64], uint32_t 
 inline unsigned la_tile_grid(int64_t tiles) { return unsigned(tiles < 2 * 148 ? tiles : 2 * 148); }
 
 // The CUDA cores while their 32 x 32 tiles (a short last chunk has fewer) take
-// one round on the SMs, or two for the chunk stage at 32 bits.  For 4 / 16 / 32
-// heads x 128 tokens x 64, in us on CUDA cores against tensor cores: chunk stage
-// 8.0 / 12.8 / 18.4 against 14.5 / 14.8 / 15.1, over Z_2^64 15.2 / 27.1 / 39.6
-// against 22.0 / 22.4 / 27.0; output stage 12.7 / 13.0 / 19.5 against 17.1 / 17.3 /
-// 17.4, over Z_2^64 23.7 / 24.1 / 41.6 against 23.0 / 23.3 / 23.4, and for 16 heads
-// x 32 tokens there 13.0 against 14.0.
-static bool ls_fits(const LaShape &s, int64_t tiles_full, int64_t tiles_last, int rounds)
+// nine quarters of a round on the SMs for the chunk stage at 32 bits, one and a half for the
+// output stage, one for either at 64.  For 4 / 16 / 32 heads x 128 tokens x 64, in us
+// on CUDA cores against tensor cores: chunk stage 7.0 / 11.1 / 17.0 against 14.6 /
+// 15.0 / 15.2, over Z_2^64 15.3 / 23.9 / 40.4 against 22.8 / 22.4 / 27.3; output stage
+// 10.0 / 10.2 / 17.8 against 17.3 / 17.4 / 17.5 (24 heads: 16.5 and 17.3), over Z_2^64
+// 22.9 / 23.1 / 41.6 against 23.2 / 23.2 / 23.4, and for 16 heads x 32 tokens there
+// 13.0 against 13.9; 16 heads x 138 tokens x 47 (304 tiles) chunk stage 11.2 and 19.7.
+static bool ls_fits(const LaShape &s, int64_t tiles_full, int64_t tiles_last, int64_t most)
 {
-    return s.bh() * ((s.chunks() - 1) * tiles_full + tiles_last) <= rounds * 148;
+    return s.bh() * ((s.chunks() - 1) * tiles_full + tiles_last) <= most;
 }
 
 template <typename T>
@@ -964,7 +985,7 @@ int la_chunk(const LaShape &s, const LaChunkArgs<T> &a, cudaStream_t st)
     const int rows = (s.len(0) + 31) / 32, tri = rows * (rows + 1) / 2;
     const int square = ((s.dk + 31) / 32) * ((s.dv + 31) / 32);
     const int last = (s.len(s.chunks() - 1) + 31) / 32;
-    if (ls_fits(s, tri + square, last * (last + 1) / 2 + square, sizeof(T) == 4 ? 2 : 1)) {
+    if (ls_fits(s, tri + square, last * (last + 1) / 2 + square, sizeof(T) == 4 ? 148 * 9 / 4 : 148)) {
         k_ls_chunk<T><<<unsigned(s.bh() * s.chunks() * (tri + square)), LA_THREADS, 0, st>>>(s, a, tri, square);
         return launched();
     }
@@ -1012,7 +1033,7 @@ int la_output(const LaShape &s, const LaOutArgs<T> &a, cudaStream_t st)
 {
     if (!s.n_out()) return DDG_OK;
     const int down = (s.len(0) + 31) / 32, across = (s.dv + 31) / 32;
-    if (ls_fits(s, down * across, (s.len(s.chunks() - 1) + 31) / 32 * across, 1)) {
+    if (ls_fits(s, down * across, (s.len(s.chunks() - 1) + 31) / 32 * across, sizeof(T) == 4 ? 148 * 3 / 2 : 148)) {
         k_ls_output<T><<<unsigned(s.bh() * s.chunks() * down * across), LA_THREADS, 0, st>>>(s, a, down, across);
         return launched();
     }
