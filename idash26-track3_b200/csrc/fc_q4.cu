@@ -6,7 +6,7 @@
 // Two kernels, both exact modulo 2^bw, so the result does not depend on how K
 // is split over lanes, warps or CTAs.
 //
-// k_q4_gemv, for one or two rows of a small product: 8-bit limb products on the CUDA cores.  x
+// k_q4_gemv, for one row or two of a smaller product: 8-bit limb products on the CUDA cores.  x
 // sits in shared memory as byte planes, four k of one limb to a word, and
 // dp4a multiplies a word by four codes: per unit of 32 codes (one 16-byte
 // load, one step)
@@ -25,7 +25,8 @@
 // cluster's shared memory.
 //
 // Measured on one B200 (graph replays, launch included): CUDA cores, 1 x 376 x
-// 1024 4.3 us and 1 x 2048 x 4096 5.4 us; tensor cores, 256 x 1024 x 512 7.1 us,
+// 1024 4.2 us, 1 x 4096 x 4096 7.7 us and 1 x 4096 x 8192 11.3 us (1.5 TB/s of codes;
+// the limb products' issue); tensor cores, 256 x 1024 x 512 7.1 us,
 // 16 x 4096 x 8192 15.0 us (16.8 MB of codes, 1.1 TB/s: bound by the expansion
 // in its sixteen warps), 2048 x 4096 x 4096 230 us (0.30 P ring flop/s, 1.2 P byte
 // products/s: tensor pipe 62 % busy, bound by shared memory).
@@ -59,9 +60,11 @@ inline GvGeom gv_geom(int K, int N, int R)
     g.L = 1;
     while (g.L < 32 && g.L < g.U) g.L *= 2;
     g.nseg = (g.U + g.L - 1) / g.L;
-    g.KS = g.nseg < 1 ? 1 : g.nseg < GV_WARPS ? g.nseg : GV_WARPS;
-    g.slots = GV_WARPS / g.KS * (32 / g.L);
-    g.blocks = (N + g.slots * R - 1) / (g.slots * R);
+    auto slots = [&](int ks) { return GV_WARPS / ks * (32 / g.L); };
+    auto blocks = [&](int ks) { return int((int64_t(N) + slots(ks) * R - 1) / (slots(ks) * R)); };
+    g.KS = 1;  // as many as leave one round of two CTAs an SM
+    while (2 * g.KS <= GV_WARPS && g.KS < g.nseg && blocks(2 * g.KS) <= 2 * 148) g.KS *= 2;
+    g.slots = slots(g.KS), g.blocks = blocks(g.KS);
     return g;
 }
 
@@ -768,10 +771,13 @@ int fc_q4(const Q4Args<T> &a, cudaStream_t st)
         return DDG_OK;
     }
     const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
-    // the CUDA cores for one or two rows while the product is small: 1 x 1024 x 1024 takes 4.4 us there and
-    // 5.5 on the tensor cores, 1 x 4096 x 4096 over Z_2^64 13.2 and 10.7
+    // The CUDA cores for one row over Z_2^32 (1 x 1024 x 1024 takes 4.4 us there and 5.6 on the tensor cores,
+    // 1 x 8192 x 8192 18.7 and 22.8), for one over Z_2^64 (twice the limb products) up to 4096 x 4096 (10.5 and
+    // 10.7; 4096 x 8192 18.2 and 16.6), for two of half that (2 x 2048 x 2048 5.9 and 6.7 over Z_2^32, 7.8 and 7.8
+    // over Z_2^64; 2 x 4096 x 4096 10.7 and 9.2).
     const uint64_t macs = uint64_t(a.M) * uint64_t(a.w.K) * uint64_t(a.w.N);
-    if (a.M <= 2 && macs * sizeof(T) <= (1u << 25) && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
+    const uint64_t most = a.M == 2 ? 1u << 26 : sizeof(T) == 8 ? 1u << 27 : ~0ull;
+    if (a.M <= 2 && macs * sizeof(T) <= most && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
         return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
     // The tile of least estimated time.  Wide tiles expand the weights fewer times
     // and split x for more outputs, narrow ones spread a small product over more

@@ -75,6 +75,14 @@ def test_fc_q4_long_reductions(ddg, cuda, bw, M, K, N):
 
 
 @pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 9000), (1, 1023, 20001), (1, 2500, 2403), (2, 1500, 3001), (2, 2100, 7),
+                                   (1, 20000, 600), (1, 30000, 50)])
+def test_fc_q4_few_rows(ddg, cuda, bw, M, K, N):
+    # one or two rows: every way of sharing K between the warps, several rounds of outputs
+    fc_case(ddg, bw, M, K, N, 64)
+
+
+@pytest.mark.parametrize("bw", [32, 64])
 @pytest.mark.parametrize("M", [1, 6, 70])
 def test_fc_q4_strided_rows_no_bias_and_in_place(ddg, cuda, bw, M):
     fc_case(ddg, bw, M, 100, 60, 32, ldx=103)
