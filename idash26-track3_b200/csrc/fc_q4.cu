@@ -25,7 +25,7 @@
 // cluster's shared memory.
 //
 // Measured on one B200 (graph replays, launch included): CUDA cores, 1 x 376 x
-// 1024 4.2 us, 1 x 4096 x 4096 7.7 us and 1 x 4096 x 8192 11.3 us (1.5 TB/s of codes;
+// 1024 4.1 us, 1 x 4096 x 4096 7.6 us and 1 x 4096 x 8192 11.2 us (1.5 TB/s of codes;
 // the limb products' issue); tensor cores, 256 x 1024 x 512 7.1 us,
 // 16 x 4096 x 8192 15.0 us (16.8 MB of codes, 1.1 TB/s: bound by the expansion
 // in its sixteen warps), 2048 x 4096 x 4096 230 us (0.30 P ring flop/s, 1.2 P byte
@@ -106,9 +106,15 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
         }
     };
 
-    // the first codes are in flight while x is split
-    Codes cur;
-    fetch(blockIdx.x, ks, cur);
+    // the first codes are in flight while x is split, then those of the next segment (two ahead took no less time)
+    Codes cur, next;
+    int fblk = blockIdx.x, fseg = ks;  // the next segment to fetch
+    auto fetch_next = [&](Codes &f) {
+        fetch(fblk, fseg, f);
+        fseg += g.KS;
+        if (fseg >= g.nseg) fseg = ks, fblk += gridDim.x;
+    };
+    fetch_next(cur);
     const int quarters = MR * g.U * 4;
     for (int i0 = warp * 32; i0 < quarters; i0 += Q4_THREADS) {  // warp-uniform: the shuffles below are whole
         const bool in = i0 + lane < quarters;
@@ -155,11 +161,7 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
 #pragma unroll
             for (int m = 0; m < MR; m++) acc[r][m] = 0;
         for (int seg = ks; seg < g.nseg; seg += g.KS) {
-            Codes next;
-            if (seg + g.KS < g.nseg)
-                fetch(blk, seg + g.KS, next);
-            else
-                fetch(blk + gridDim.x, ks, next);
+            fetch_next(next);
             const int u = seg * g.L + li;
             if (active && u < g.U) {
 #pragma unroll
@@ -771,7 +773,7 @@ int fc_q4(const Q4Args<T> &a, cudaStream_t st)
         return DDG_OK;
     }
     const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
-    // The CUDA cores for one row over Z_2^32 (1 x 1024 x 1024 takes 4.4 us there and 5.6 on the tensor cores,
+    // The CUDA cores for one row over Z_2^32 (1 x 1024 x 1024 takes 4.2 us there and 5.6 on the tensor cores,
     // 1 x 8192 x 8192 18.7 and 22.8), for one over Z_2^64 (twice the limb products) up to 4096 x 4096 (10.5 and
     // 10.7; 4096 x 8192 18.2 and 16.6), for two of half that (2 x 2048 x 2048 5.9 and 6.7 over Z_2^32, 7.8 and 7.8
     // over Z_2^64; 2 x 4096 x 4096 10.7 and 9.2).
