@@ -644,29 +644,29 @@ __global__ void __launch_bounds__(Q4_THREADS) k_q4_empty(const __grid_constant__
 // reach the group's largest weight (at most 4095, beyond which codes saturate),
 // codes rounded to nearest
 __global__ void __launch_bounds__(256)
-    k_q4_quantize(int K, int N, int group, const int64_t *w, uint8_t *q, uint16_t *step, int64_t row_bytes)
+    k_q4_quantize(int64_t K, int64_t N, int64_t group, const int64_t *w, uint8_t *q, uint16_t *step, int64_t row_bytes)
 {
+    // K and group go up to the largest int, and their sum beyond it
     const int64_t e = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    const int ng = (K + group - 1) / group;
-    if (e >= int64_t(ng) * N) return;
-    const int64_t n = e % N;
-    const int k0 = int(e / N) * group, k1 = K - k0 < group ? K : k0 + group;
+    const int64_t ng = (K + group - 1) / group;
+    if (e >= ng * N) return;
+    const int64_t n = e % N, k0 = e / N * group, k1 = K - k0 < group ? K : k0 + group;
     auto mag = [](int64_t v) { return v < 0 ? uint64_t(0) - uint64_t(v) : uint64_t(v); };
     uint64_t top = 0;
-    for (int k = k0; k < k1; k++) {
-        const uint64_t a = mag(w[int64_t(k) * N + n]);
+    for (int64_t k = k0; k < k1; k++) {
+        const uint64_t a = mag(w[k * N + n]);
         top = a > top ? a : top;
     }
     const uint64_t fit = top / 7 + (top % 7 ? 1 : 0);
     const uint64_t s = fit < 1 ? 1 : fit > uint64_t(Q4_STEP_MAX) ? uint64_t(Q4_STEP_MAX) : fit;
     step[e] = uint16_t(s);
-    const int kend = k1 == K ? int(2 * row_bytes) : k1;  // the row's padding holds zero weights
-    for (int k = k0; k < kend; k += 2) {
+    const int64_t kend = k1 == K ? 2 * row_bytes : k1;  // the row's padding holds zero weights
+    for (int64_t k = k0; k < kend; k += 2) {
         uint32_t byte = 0;
         for (int i = 0; i < 2; i++) {
             uint32_t code = 8;
             if (k + i < K) {
-                const int64_t v = w[int64_t(k + i) * N + n];
+                const int64_t v = w[(k + i) * N + n];
                 const uint64_t a = mag(v);
                 const uint32_t r = a >= 8 * s ? 8 : uint32_t((2 * a + s) / (2 * s));
                 code = v < 0 ? 8 - r : 8 + (r > 7 ? 7 : r);
