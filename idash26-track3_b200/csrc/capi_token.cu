@@ -185,7 +185,7 @@ int ddg_decay_table(int bw, int scale, int heads, int n, const double *h_lambda,
         DDG_CHECK(h_lambda[h] >= 0.0 && h_lambda[h] <= 1.0, DDG_ERR_ARG, "decay %d is not in [0, 1]", h);
     for (int h = 0; h < heads; h++) {
         double p = std::ldexp(1.0, scale);
-        for (int i = 0; i <= n; i++, p *= h_lambda[h]) {
+        for (int64_t i = 0; i <= n; i++, p *= h_lambda[h]) {  // n may be the largest int
             const uint64_t v = uint64_t(std::llround(p));
             const int64_t at = int64_t(h) * (int64_t(n) + 1) + i;
             if (bw == 32)

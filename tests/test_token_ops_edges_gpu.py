@@ -59,3 +59,41 @@ def test_q4_quantize_of_the_longest_column(ddg, cuda):
     last, tail = int(step[-1]), q[-2:].tolist()
     assert (other_codes, other_steps, last) == (0, 0, 3)
     assert tail == [0x18, 0x8B]
+
+
+# ---------------------------------------------------------------- linear attention
+
+def test_linattn_longest_table_of_powers(ddg, cuda):
+    """pow_n = 2^31 - 1: the second head's powers start 2^31 elements into the table."""
+    import torch
+
+    T, dk, dv = 5, 4, 8
+    table = torch.zeros(1 << 32, dtype=torch.int32, device="cuda")
+    for bw, width in ((32, 4), (64, 8)):  # over Z_2^64 one head's table is what fits here
+        H = 2 if bw == 32 else 1
+        rng = np.random.default_rng(bw)
+        few = rnd(rng, bw, H, T + 1)
+        view = table.view(torch.uint8).view(H, -1)
+        for h in range(H):
+            view[h, :few[h].nbytes] = to_dev(few[h])
+        s, one = R.Shape(1, H, T, dk, dv, 2), R.Shape(1, H, 1, dk, dv, 2)
+        sh, sh1 = (ddg.LinattnShape(1, H, t, dk, dv, 2, (1 << 31) - 1) for t in (T, 1))
+        x, ps, s0 = rnd(rng, bw, 1, T, s.width), rnd(rng, bw, s.n_ps), rnd(rng, bw, s.n_state)
+        dx, dps, ds0 = to_dev(x), to_dev(ps), to_dev(s0)
+        o1, o2 = dev_bytes(2 * s.n_decayed * width), dev_bytes(s.n_ps * width)
+        torch.cuda.synchronize()
+        ddg.linattn_decay(bw, sh, s.width, ptr(table), ptr(dx), ptr(o1))
+        ddg.linattn_carry(bw, sh, ptr(table), ptr(dps), ptr(ds0), ptr(o2))
+        assert np.array_equal(from_dev(o1, ring_dt(bw), 2 * s.n_decayed), R.ring(R.decay(s, few, x), bw))
+        assert np.array_equal(from_dev(o2, ring_dt(bw), s.n_ps), R.ring(R.carry(s, few, ps, s0), bw))
+        x, rx, rs, nyw = rnd(rng, bw, 1, 1, s.width), rnd(rng, bw, 1, 1, s.width), rnd(rng, bw, s.n_state), H * (dv + 1)
+        z, yw, ryw, zo = (rnd(rng, bw, n) for n in (s.n_state + nyw, nyw, nyw, H * dv))
+        dx, drx, drs, dz, dyw, dryw, dzo = (to_dev(i) for i in (x, rx, rs, z, yw, ryw, zo))
+        torch.cuda.synchronize()
+        ddg.linattn_step_share(bw, 0, sh1, s.width, ptr(table), ptr(dx), ptr(drx), ptr(ds0), ptr(drs), ptr(dz), ptr(dz))
+        ddg.linattn_step_output_share(bw, 0, sh1, s.width, ptr(table), ptr(dx), ptr(drx), ptr(dyw), ptr(dryw), ptr(dzo),
+                                      ptr(dzo))
+        assert np.array_equal(from_dev(dz, z.dtype, z.size),
+                              R.ring(R.step_share(one, 0, few[:, 1], x, rx, s0, rs) + z, bw))
+        assert np.array_equal(from_dev(dzo, z.dtype, zo.size),
+                              R.ring(R.step_output_share(one, 0, few[:, 1], x, rx, yw, ryw) + zo, bw))
