@@ -121,6 +121,7 @@ int run_eval(ddg_party *h, ddg_cursor *cur, int batch, F &&body)
     return DDG_OK;
 }
 
+// weights: the call reads the affinity model's (its layers' matrices or the D^-1/2 table)
 int eval_ready(ddg_party *h, ddg_cursor *cur, int batch, bool weights = true)
 {
     DDG_CHECK(h && cur, DDG_ERR_ARG, "null party or cursor");
@@ -310,7 +311,7 @@ int ddg_op_matmul_eval(ddg_party *h, ddg_cursor *cur, int batch, int k, ddg_wire
 int ddg_op_mul_eval(ddg_party *h, ddg_cursor *cur, int bcast, int rows, int cols, ddg_wire *a, ddg_wire *b,
                     int trunc, ddg_wire *out)
 {
-    DDG_TRY(eval_ready(h, cur, 1));
+    DDG_TRY(eval_ready(h, cur, 1, false));
     DDG_TRY(check_wires({a, b, out, out ? out->d_value : nullptr}));
     DDG_CHECK(bcast >= BC_NONE && bcast <= BC_COL, DDG_ERR_ARG, "bcast %d out of range", bcast);
     DDG_CHECK(bcast == BC_NONE || (rows > 0 && cols > 0 && a->n % (uint64_t(rows) * cols) == 0), DDG_ERR_ARG,
@@ -329,7 +330,7 @@ int ddg_op_mul_eval(ddg_party *h, ddg_cursor *cur, int bcast, int rows, int cols
 
 int ddg_op_gate_eval(ddg_party *h, ddg_cursor *cur, int kind, ddg_wire *x, ddg_wire *out)
 {
-    DDG_TRY(eval_ready(h, cur, 1));
+    DDG_TRY(eval_ready(h, cur, 1, false));
     DDG_TRY(check_wires({x, out, out ? out->d_value : nullptr}));
     DDG_TRY(check_gate_kind(kind, h->P.bw, h->P.s));
 #define BODY(T)                         \
@@ -384,7 +385,7 @@ int ddg_op_concat_protein_eval(ddg_party *h, ddg_cursor *cur, int batch, ddg_wir
 
 int ddg_op_output_eval(ddg_party *h, ddg_cursor *cur, int batch, ddg_wire *o, int64_t *h_out_raw, double *h_affinity)
 {
-    DDG_TRY(eval_ready(h, cur, batch));
+    DDG_TRY(eval_ready(h, cur, batch, false));
     DDG_TRY(check_wires({o}));
     DDG_CHECK(o->n == uint64_t(batch), DDG_ERR_ARG, "output wire holds %llu values for batch %d",
               (unsigned long long)o->n, batch);

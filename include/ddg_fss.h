@@ -420,7 +420,9 @@ typedef struct ddg_mask_wire {
  * (batch,138,94), GCN layer l output (batch,138,{188,282,376}[l]), max-pool
  * input (batch,138,376) and output (batch,376), FC layer l (rows x in) ->
  * (rows x out) with (in,out) of weights.bin layer l, concat (batch,128) ->
- * (batch,256). */
+ * (batch,256).  ddg_op_input_eval, ddg_op_mul_eval, ddg_op_gate_eval and
+ * ddg_op_output_eval take any sizes and need no ddg_party_set_weights; the
+ * others refuse a party without weights (DDG_ERR_STATE). */
 /* a secret-shared input leaf: own share + own mask share, opened
  * (registerLeaf + revealIfLeaf, ddg_orca_base.h:72-80) */
 int ddg_op_input_eval(ddg_party *party, ddg_cursor *cur, uint64_t n, const void *d_share, ddg_wire *out);
@@ -453,7 +455,7 @@ int ddg_op_fc_eval(ddg_party *party, ddg_cursor *cur, int layer, int rows, int a
 int ddg_op_concat_protein_eval(ddg_party *party, ddg_cursor *cur, int batch, ddg_wire *d2,
                                const void *d_protein_share, ddg_wire *out);
 /* Backend<T>::output (ddg_orca_base.h:296-302): unmask, shift by scale; the
- * same outputs as ddg_forward_eval */
+ * same outputs as ddg_forward_eval.  batch is the wire's number of values */
 int ddg_op_output_eval(ddg_party *party, ddg_cursor *cur, int batch, ddg_wire *o, int64_t *h_out_raw,
                        double *h_affinity);
 

@@ -97,3 +97,76 @@ def test_linattn_longest_table_of_powers(ddg, cuda):
                               R.ring(R.step_share(one, 0, few[:, 1], x, rx, s0, rs) + z, bw))
         assert np.array_equal(from_dev(dzo, z.dtype, zo.size),
                               R.ring(R.step_output_share(one, 0, few[:, 1], x, rx, yw, ryw) + zo, bw))
+
+
+# ---------------------------------------------------------------- as wires
+
+@pytest.mark.parametrize("bw", [32, 64])
+def test_token_model_result_is_read_without_affinity_weights(ddg, synth, cuda, bw):
+    """Input -> 4-bit layer -> gate -> product of wires -> output on parties that hold no affinity weights; the calls
+    that read those weights still refuse."""
+    from tests.test_layers_gpu import Bufs, run_both
+
+    L, dt, n = ddg.lib(), ring_dt(bw), 24
+    rng = np.random.default_rng(bw)
+    K, N, rows = 40, 12, 2
+    one = 1 << S
+    w = np.round(rng.normal(0, 0.3, (K, N)) * one).astype(np.int64)
+    x = np.round(rng.uniform(-1, 1, (rows, K)) * one).astype(np.int64)
+    y = np.round(rng.uniform(0, 6, (rows, N)) * one).astype(np.int64)
+    code, step = R.q4_quantize(w, 32)
+    act = np.maximum((x @ R.q4_weights(code, step, 32)) >> S, 0)
+    want = ((act * y) >> S).reshape(-1)
+    assert np.abs(act * y).max() < 1 << (bw - 2) and want.any()
+    dw, dq, ds = to_dev(w), dev_bytes(N * 16 * ((K + 31) // 32)), dev_bytes(step.size * 2)
+    ddg.q4_quantize(K, N, 32, ptr(dw), ptr(dq), ptr(ds))
+    q4 = ddg.Q4Weights(K, N, 32, ptr(dq), ptr(ds), None)
+
+    kb = 1 << 20
+    keys = [dev_bytes(kb) for _ in range(2)]
+    d = ddg.Dealer(bw, S, 0, 5, synth.weights_blob(synth.quantize_weights(synth.affinity_weights(5), S)))
+    d.bind_keys(ptr(keys[0]), ptr(keys[1]), kb)
+    bufs = [Bufs(bw // 8) for _ in range(3)]
+    c, mw = ddg.Cursor(), lambda k: bufs[2].mask_wire(ddg, k)
+    X, Y, Z, A, P = mw(x.size), mw(n), mw(n), mw(n), mw(n)
+    for st in (L.ddg_op_input_keygen(d.h, c, x.size, X), L.ddg_op_input_keygen(d.h, c, n, Y),
+               L.ddg_op_fc_q4_keygen(d.h, c, q4, rows, ddg.ACT_NONE, X, Z),
+               L.ddg_op_gate_keygen(d.h, c, ddg.GATE_RELU_ARS, Z, A),
+               L.ddg_op_mul_keygen(d.h, c, 0, 0, 0, A, Y, 0, P), L.ddg_op_output_keygen(d.h, c, P)):
+        ddg.check(st)
+    end = c.offset
+
+    def split(v):
+        a = rnd(rng, bw, v.size)
+        return to_dev(a), to_dev((R.ring(v.reshape(-1).view(np.uint64), bw) - a).astype(dt))
+
+    sx, sy = split(x), split(y)
+    ps = [ddg.Party(p, bw, S, 0) for p in (0, 1)]
+    for p, k in zip(ps, keys):
+        p.bind_keys(ptr(k), kb)
+    ddg.pair_local(ps[0], ps[1])
+    got = [None, None]
+
+    def side(p):
+        c, wi, h = ddg.Cursor(), lambda k: bufs[p].wire(ddg, k), ps[p].h
+        X, Y, Z, A, P = wi(x.size), wi(n), wi(n), wi(n), wi(n)
+        ddg.check(L.ddg_op_input_eval(h, c, x.size, ptr(sx[p]), X))
+        ddg.check(L.ddg_op_input_eval(h, c, n, ptr(sy[p]), Y))
+        ddg.check(L.ddg_op_fc_q4_eval(h, c, q4, rows, ddg.ACT_NONE, X, Z))
+        ddg.check(L.ddg_op_gate_eval(h, c, ddg.GATE_RELU_ARS, Z, A))
+        ddg.check(L.ddg_op_mul_eval(h, c, 0, 0, 0, A, Y, 0, P))
+        raw = np.zeros(n, np.int64)
+        ddg.check(L.ddg_op_output_eval(h, c, n, P, raw.ctypes.data, None))
+        assert c.offset == end
+        # what reads the affinity weights
+        big = wi(138 * 376)
+        assert L.ddg_adjnorm_eval(h, c, 1, ptr(sx[p]), big) == 5
+        assert L.ddg_op_fc_eval(h, c, 8, 1, 0, wi(256), wi(1)) == 5
+        assert L.ddg_gcn_layer_eval(h, c, 0, 1, wi(138 * 138), wi(138 * 94), big) == 5
+        got[p] = raw
+
+    run_both(lambda: side(0), lambda: side(1))
+    for p in (0, 1):
+        assert np.array_equal(got[p], want)
+        ps[p].close()
+    d.close()
