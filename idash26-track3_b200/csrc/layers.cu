@@ -179,6 +179,22 @@ int check_gate_kind(int kind, int bw, int s)
     return DDG_OK;
 }
 
+// the token model's kernels read ring arrays in whole elements; null stands for "none" and passes
+int check_elements(int bw, std::initializer_list<const void *> ptrs)
+{
+    for (const void *p : ptrs)
+        DDG_CHECK(reinterpret_cast<uintptr_t>(p) % uintptr_t(bw / 8) == 0, DDG_ERR_ARG, "misaligned ring array");
+    return DDG_OK;
+}
+int check_elements(int bw, const ddg_wire *w)
+{
+    return w ? check_elements(bw, {w->d_value, w->d_mask_share}) : DDG_OK;
+}
+int check_elements(int bw, const ddg_mask_wire *w)
+{
+    return w ? check_elements(bw, {w->d_mask, w->d_share0, w->d_share1}) : DDG_OK;
+}
+
 // the token model's layers: the ring and scale of the floors, then the layer's own sizes
 int check_floor(int bw, int s)
 {
@@ -205,8 +221,19 @@ int check_la_layer(const ddg_linattn_shape *p, int bw, int s, bool step, LaShape
 }
 
 template <class W>
-int check_la_wires(const LaShape &s, const W *qkv, const W *s0)
+int check_fc_q4_wires(const ddg_q4_weights *w, int bw, int rows, const W *x)
 {
+    DDG_CHECK(x->n == uint64_t(rows) * w->K, DDG_ERR_ARG, "FC input is not %d x %d", rows, w->K);
+    DDG_TRY(check_elements(bw, {w->d_bias2s}));
+    return check_elements(bw, x);
+}
+
+template <class W>
+int check_la_wires(const LaShape &s, int bw, const void *d_pow, const W *qkv, const W *s0)
+{
+    DDG_TRY(check_elements(bw, {d_pow}));
+    DDG_TRY(check_elements(bw, qkv));
+    DDG_TRY(check_elements(bw, s0));
     DDG_CHECK(qkv->n == uint64_t(s.n_qkv()), DDG_ERR_ARG, "the q|k|v wire holds %llu elements, not %lld",
               (unsigned long long)qkv->n, (long long)s.n_qkv());
     DDG_CHECK(!s0 || s0->n == uint64_t(s.n_state()), DDG_ERR_ARG, "the state wire holds %llu elements, not %lld",
@@ -618,7 +645,7 @@ int ddg_op_fc_q4_eval(ddg_party *h, ddg_cursor *cur, const ddg_q4_weights *w, in
     DDG_TRY(eval_ready(h, cur, 1, false));
     DDG_TRY(check_wires({x, out, x ? x->d_value : nullptr, out ? out->d_value : nullptr}));
     DDG_TRY(check_fc_q4(w, h->P.bw, h->P.s, rows, act));
-    DDG_CHECK(x->n == uint64_t(rows) * w->K, DDG_ERR_ARG, "FC input is not %d x %d", rows, w->K);
+    DDG_TRY(check_fc_q4_wires(w, h->P.bw, rows, x));
 #define BODY(T)                                                    \
     Tn<T> X = tn_of<T>(x);                                         \
     Tn<T> y = fc_q4_layer<T>(e, X, q4_of<T>(w), rows, act);        \
@@ -633,7 +660,7 @@ int ddg_op_fc_q4_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_q4_weights *w,
     DDG_TRY(keygen_ready(d, cur, 1));
     DDG_TRY(check_wires({x, out, x ? x->d_mask : nullptr, out ? out->d_mask : nullptr}));
     DDG_TRY(check_fc_q4(w, d->bw, d->s, rows, act));
-    DDG_CHECK(x->n == uint64_t(rows) * w->K, DDG_ERR_ARG, "FC input is not %d x %d", rows, w->K);
+    DDG_TRY(check_fc_q4_wires(w, d->bw, rows, x));
 #define BODY(T)                                                    \
     Tn<T> X = tn_of<T>(x);                                         \
     Tn<T> y = fc_q4_layer<T>(e, X, q4_of<T>(w), rows, act);        \
@@ -672,7 +699,7 @@ int ddg_linattn_eval(ddg_party *h, ddg_cursor *cur, const ddg_linattn_shape *sha
     DDG_TRY(check_la_layer(shape, h->P.bw, h->P.s, false, &s));
     DDG_TRY(check_wires({d_pow, qkv, out, state_out, qkv ? qkv->d_value : nullptr, out ? out->d_value : nullptr,
                          state_out ? state_out->d_value : nullptr, s0 ? s0->d_value : d_pow}));
-    DDG_TRY(check_la_wires(s, qkv, s0));
+    DDG_TRY(check_la_wires(s, h->P.bw, d_pow, qkv, s0));
     return DDG_DISPATCH_EVAL(h, cur, s.B, LA_BODY);
 }
 
@@ -684,7 +711,7 @@ int ddg_linattn_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_linattn_shape *
     DDG_TRY(check_la_layer(shape, d->bw, d->s, false, &s));
     DDG_TRY(check_wires({d_pow, qkv, out, state_out, qkv ? qkv->d_mask : nullptr, out ? out->d_mask : nullptr,
                          state_out ? state_out->d_mask : nullptr, s0 ? s0->d_mask : d_pow}));
-    DDG_TRY(check_la_wires(s, qkv, s0));
+    DDG_TRY(check_la_wires(s, d->bw, d_pow, qkv, s0));
     return DDG_DISPATCH_KEYGEN(d, cur, s.B, LA_BODY);
 }
 #undef LA_BODY
@@ -717,7 +744,7 @@ int ddg_linattn_step_eval(ddg_party *h, ddg_cursor *cur, const ddg_linattn_shape
     DDG_TRY(check_la_layer(shape, h->P.bw, h->P.s, true, &s));
     DDG_TRY(check_wires({d_pow, qkv, s_in, out, state_out, qkv ? qkv->d_value : nullptr, s_in ? s_in->d_value : nullptr,
                          out ? out->d_value : nullptr, state_out ? state_out->d_value : nullptr}));
-    DDG_TRY(check_la_wires(s, qkv, s_in));
+    DDG_TRY(check_la_wires(s, h->P.bw, d_pow, qkv, s_in));
     return DDG_DISPATCH_EVAL(h, cur, s.B, LA_BODY);
 }
 
@@ -729,7 +756,7 @@ int ddg_linattn_step_keygen(ddg_dealer *d, ddg_cursor *cur, const ddg_linattn_sh
     DDG_TRY(check_la_layer(shape, d->bw, d->s, true, &s));
     DDG_TRY(check_wires({d_pow, qkv, s_in, out, state_out, qkv ? qkv->d_mask : nullptr, s_in ? s_in->d_mask : nullptr,
                          out ? out->d_mask : nullptr, state_out ? state_out->d_mask : nullptr}));
-    DDG_TRY(check_la_wires(s, qkv, s_in));
+    DDG_TRY(check_la_wires(s, d->bw, d_pow, qkv, s_in));
     return DDG_DISPATCH_KEYGEN(d, cur, s.B, LA_BODY);
 }
 #undef LA_BODY

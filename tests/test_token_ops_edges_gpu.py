@@ -170,3 +170,52 @@ def test_token_model_result_is_read_without_affinity_weights(ddg, synth, cuda, b
         assert np.array_equal(got[p], want)
         ps[p].close()
     d.close()
+
+
+@pytest.mark.parametrize("bw,off", [(32, 2), (64, 4)])
+def test_wire_calls_refuse_misaligned_arrays(ddg, synth, cuda, bw, off):
+    """A wire, bias or table of powers off its element boundary would fault in a kernel: refused before any work, on
+    the dealer and on a party, the cursors unmoved."""
+    from tests.test_layers_gpu import Bufs
+
+    L, kb = ddg.lib(), 1 << 18
+    keys = [dev_bytes(kb) for _ in range(2)]
+    d = ddg.Dealer(bw, S, 0, 1, synth.weights_blob(synth.quantize_weights(synth.affinity_weights(5), S)))
+    d.bind_keys(ptr(keys[0]), ptr(keys[1]), kb)
+    ps = [ddg.Party(p, bw, S, 0) for p in (0, 1)]
+    for p, k in zip(ps, keys):
+        p.bind_keys(ptr(k), kb)
+    ddg.pair_local(ps[0], ps[1])
+    b, q = Bufs(bw // 8), dev_bytes(1 << 16)
+    sh, sh1, nq, ns = ddg.LinattnShape(1, 2, 3, 4, 5, 2, 3), ddg.LinattnShape(1, 2, 1, 4, 5, 2, 3), 78, 40
+    good = ddg.Q4Weights(32, 8, 32, ptr(q), ptr(q), ptr(q))
+    bad_bias = ddg.Q4Weights(32, 8, 32, ptr(q), ptr(q), ptr(q) + off)
+    p, bad = ptr(q), ptr(q) + off
+
+    def calls(h, c, kind, new, wire):
+        fc, pr, st = (getattr(L, f"ddg_{n}_{kind}") for n in ("op_fc_q4", "linattn", "linattn_step"))
+        yield fc(h, c, bad_bias, 2, 0, new(64), new(16))
+        for x in wire(64):
+            yield fc(h, c, good, 2, 0, x, new(16))
+        yield pr(h, c, sh, bad, new(nq), None, new(30), new(ns))
+        yield st(h, c, sh1, bad, new(nq // 3), new(ns), new(10), new(ns))
+        for x in wire(nq):
+            yield pr(h, c, sh, p, x, None, new(30), new(ns))
+        for x in wire(nq // 3):
+            yield st(h, c, sh1, p, x, new(ns), new(10), new(ns))
+        for x in wire(ns):
+            yield pr(h, c, sh, p, new(nq), x, new(30), new(ns))
+            yield st(h, c, sh1, p, new(nq // 3), x, new(10), new(ns))
+
+    c = ddg.Cursor()
+    masks = lambda n: [ddg.MaskWire(*a) for a in ((bad, n, None, None), (p, n, bad, p), (p, n, p, bad))]  # noqa: E731
+    said = lambda it: {(st, L.ddg_last_error()) for st in it}  # noqa: E731
+    refused = {(1, b"misaligned ring array")}
+    assert said(calls(d.h, c, "keygen", lambda n: b.mask_wire(ddg, n), masks)) == refused
+    assert (c.offset, c.ops) == (0, 0)
+    values = lambda n: [ddg.Wire(bad, n, None), ddg.Wire(p, n, bad)]  # noqa: E731
+    for party in ps:
+        assert said(calls(party.h, c, "eval", lambda n: b.wire(ddg, n), values)) == refused and c.offset == 0
+    for party in ps:
+        party.close()
+    d.close()
