@@ -16,7 +16,7 @@ inline int tma_map_2d(CUtensorMap *map, const void *base, int elem_bytes, uint64
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static Encode encode = nullptr;
+    static thread_local Encode encode = nullptr;  // parties of one process call from threads of their own
     if (!encode) {
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q;
