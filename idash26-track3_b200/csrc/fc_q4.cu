@@ -270,8 +270,10 @@ struct QtShape {
     static_assert(UNITS <= THREADS && THREADS % XROW == 0 && (ITEMS % THREADS == 0 || XPT == 1), "x items");
 };
 
+// (.aligned: the lanes of a warp arrive together, whatever branches they come from)
 __device__ __forceinline__ void cluster_sync()
 {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -538,6 +540,7 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
             }
             proxy_fence();
             if constexpr (S::A_TMEM) {
+                __syncwarp();  // the wait is .aligned, and the lanes' loads of steps and x are their own
                 tmem_st_wait();
                 tc_fence_before();
             }
@@ -625,6 +628,7 @@ __global__ void __launch_bounds__(QtShape<T, MT, NA>::THREADS + 64, 1)
         }
     }
     if (split) cluster_sync();  // nobody leaves while its sums are read
+    __syncwarp();               // lanes without an output of theirs are here first
     if (warp == 0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::COLS) : "memory");

@@ -278,7 +278,12 @@ struct LtTile {
     int64_t at, stride;
 };
 
-__device__ __forceinline__ void expander_sync() { asm volatile("bar.sync 1, %0;" ::"n"(LT_THREADS) : "memory"); }
+// (bar.sync is .aligned: the lanes of a warp arrive together, whatever rows and columns they have stored)
+__device__ __forceinline__ void expander_sync()
+{
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(LT_THREADS) : "memory");
+}
 
 // Tiles first, first + step, .. below `tiles`; tile_of(index) describes one.
 // beaver: with the mask-share products (odd K-steps are -[a] . b), else the
