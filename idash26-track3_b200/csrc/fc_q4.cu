@@ -767,9 +767,13 @@ static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
 }
 
 template <typename T>
-int fc_q4(const Q4Args<T> &a, cudaStream_t st)
+int fc_q4(const Q4Args<T> &args, cudaStream_t st)
 {
+    Q4Args<T> a = args;
     if (int64_t(a.M) * a.w.N == 0) return DDG_OK;
+    // a single row's stride is not used: any value goes, also one that no tensor map takes
+    constexpr int V = 16 / int(sizeof(T));
+    if (a.M == 1) a.ldx = (a.w.K + V - 1) / V * V;
     if (a.w.K == 0) {
         k_q4_empty<T><<<148, Q4_THREADS, 0, st>>>(a);
         note_launch();

@@ -61,6 +61,34 @@ def test_q4_quantize_of_the_longest_column(ddg, cuda):
     assert tail == [0x18, 0x8B]
 
 
+@pytest.mark.parametrize("bw,K,N", [(32, 100, 60), (64, 100, 60), (64, 4100, 4200), (32, 130000, 70)])
+def test_stride_of_a_single_row_is_not_used(ddg, cuda, bw, K, N):
+    """With one row nothing lies a stride away: any ldx >= K gives the same product (CUDA and tensor cores)."""
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(K)
+    dt = torch.int32 if bw == 32 else torch.int64
+    row = 16 * ((K + 31) // 32)
+    q = torch.randint(0, 256, (N, row), device="cuda", generator=g).to(torch.uint8)
+    st = torch.randint(0, 4096, ((K + 31) // 32, N), device="cuda", generator=g).to(torch.int16)
+    x = torch.randint(-(1 << (bw - 1)), (1 << (bw - 1)) - 1, (1, K), dtype=dt, device="cuda", generator=g)
+    C = torch.zeros(1, N, dtype=dt, device="cuda")
+    outs = []
+    for ldx in (K, K + 1, 1 << 40, (1 << 62) + 1, (1 << 63) - 1):
+        out = torch.empty(1, N, dtype=dt, device="cuda")
+        torch.cuda.synchronize()
+        ddg.fc_q4_share(bw, 0, 1, ddg.Q4Weights(K, N, 32, ptr(q), ptr(st), None), ptr(x), ldx, ptr(C), ptr(out))
+        outs.append(out)
+    code = torch.stack((q & 15, q >> 4), 2).reshape(N, -1)[:, :K].double() - 8
+    W = code.t() * st.double().repeat_interleave(32, 0)[:K]
+    want = torch.zeros(1, N, dtype=torch.int64, device="cuda")
+    for i in range(bw // 16):  # 2^16 x 2^15 x K < 2^53: exact
+        want = want + (torch.matmul(((x.long() >> (16 * i)) & 0xFFFF).double(), W).long() << (16 * i))
+    same = [bool(torch.equal(out, want.to(dt))) for out in outs]
+    assert all(same)
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
 # ---------------------------------------------------------------- linear attention
 
 def test_linattn_longest_table_of_powers(ddg, cuda):
