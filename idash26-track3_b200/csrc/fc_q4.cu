@@ -39,40 +39,10 @@ namespace ddg {
 
 namespace {
 
-constexpr int Q4_THREADS = 256;
-
 // ------------------------------------------------------------------ one or two rows
 
-constexpr int GV_WARPS = Q4_THREADS / 32;
 template <typename T>
-constexpr int GV_R = sizeof(T) == 4 ? 4 : 2;  // outputs per lane group and pass (registers: P limb sums each)
-constexpr uint64_t GV_SMEM_MAX = 96 * 1024;
-
-// units of 32 k; a group of L lanes takes one unit each, KS warps of the CTA split the units
-struct GvGeom {
-    int U, L, nseg, KS, slots, blocks;
-};
-
-inline GvGeom gv_geom(int K, int N, int R)
-{
-    GvGeom g;
-    g.U = (K + 31) / 32;
-    g.L = 1;
-    while (g.L < 32 && g.L < g.U) g.L *= 2;
-    g.nseg = (g.U + g.L - 1) / g.L;
-    auto slots = [&](int ks) { return GV_WARPS / ks * (32 / g.L); };
-    auto blocks = [&](int ks) { return int((int64_t(N) + slots(ks) * R - 1) / (slots(ks) * R)); };
-    g.KS = 1;  // as many as leave one round of two CTAs an SM
-    while (2 * g.KS <= GV_WARPS && g.KS < g.nseg && blocks(2 * g.KS) <= 2 * 148) g.KS *= 2;
-    g.slots = slots(g.KS), g.blocks = blocks(g.KS);
-    return g;
-}
-
-template <typename T>
-uint64_t gv_smem(const GvGeom &g, int rows)
-{
-    return uint64_t(rows) * g.U * (32 * sizeof(T) + sizeof(T)) + uint64_t(GV_WARPS) * 32 * GV_R<T> * rows * sizeof(T);
-}
+constexpr int GV_R = gv_outputs(int(sizeof(T)));
 
 template <typename T, int MR>
 __global__ void __launch_bounds__(Q4_THREADS, 2)
@@ -228,7 +198,6 @@ __global__ void __launch_bounds__(Q4_THREADS, 2)
 
 // ------------------------------------------------------------------ more rows: tensor cores
 
-constexpr int QT_MAX_K = Q4_MAX_K / 8;     // k per CTA: a column's sum, 2 * 255^2 * K, stays below 2^32
 // operands lie in 16-byte chunks of 8 k, chunk-major: rows 16 bytes apart,
 // chunks of A 2048 and of B 16 NB + 16 bytes apart (the pad spreads the chunks
 // of one row, written by neighbouring lanes, over the banks)
@@ -711,26 +680,14 @@ static int launch_gemv(const Q4Args<T> &a, cudaStream_t st)
     DDG_TRY(q4_smem_limit(kern, GV_SMEM_MAX, configured));
     // two CTAs an SM, each splitting x once for all its outputs
     const int grid = g.blocks < 2 * 148 ? g.blocks : 2 * 148;
-    kern<<<grid, Q4_THREADS, gv_smem<T>(g, MR), st>>>(a, g, int64_t(q4_row_bytes(a.w.K)), q4_vec(a));
+    kern<<<grid, Q4_THREADS, gv_smem(g, MR, int(sizeof(T))), st>>>(a, g, int64_t(q4_row_bytes(a.w.K)), q4_vec(a));
     note_launch();
     DDG_CUDA(cudaGetLastError());
     return DDG_OK;
 }
 
-// CTAs of a cluster that K is split over: while that leaves every CTA resident
-// at once and two stages each, and for as long as a CTA's sums need it.
-// Clusters of four: of eight, only 15 fit the device at a time (256 CTAs of a
-// 4 x 4096 x 4096 product took three rounds).
-static int qt_split(int kc, int na, int K, int64_t ctas)
-{
-    int split = 1;
-    while (na == 1 && split < 4 && ctas * split * 2 <= 148 && K >= 4 * kc * split) split *= 2;
-    while (na == 1 && split < 8 && int64_t(K) > int64_t(QT_MAX_K) * split) split *= 2;
-    return split;
-}
-
 template <typename T, int MT, int NA>
-static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
+static int launch_tc_q4(const Q4Args<T> &a, int split, cudaStream_t st)
 {
     using S = QtShape<T, MT, NA>;
     static thread_local int configured[64];
@@ -740,11 +697,7 @@ static int launch_tc_q4(const Q4Args<T> &a, cudaStream_t st)
     DDG_TRY(ring_gemm_err_word(&err));
     const int nkc = (a.w.K + S::KC - 1) / S::KC;
     const int64_t gn = (int64_t(a.w.N) + NA * TC_BM - 1) / (NA * TC_BM), gm = (int64_t(a.M) + MT - 1) / MT;
-    DDG_CHECK(gm <= 65535, DDG_ERR_ARG, "fc_q4: %d rows are too many for one call", a.M);
-    const int split = qt_split(S::KC, NA, a.w.K, gn * gm);
-    const int most = QT_MAX_K / S::KC;
-    DDG_CHECK(nkc <= most * split, DDG_ERR_ARG, "fc_q4: K = %d is too long (at most %d)", a.w.K, 8 * QT_MAX_K);
-    const int per = nkc ? (nkc + split - 1) / split : 1;
+    const int per = (nkc + split - 1) / split;
     const int vec = q4_vec(a);
     const uint32_t gd = uint32_t(a.w.group / 32);
     const uint32_t magic = gd == 1 ? 0 : uint32_t((uint64_t(1) << 32) / gd + 1);
@@ -774,47 +727,24 @@ int fc_q4(const Q4Args<T> &args, cudaStream_t st)
     // a single row's stride is not used: any value goes, also one that no tensor map takes
     constexpr int V = 16 / int(sizeof(T));
     if (a.M == 1) a.ldx = (a.w.K + V - 1) / V * V;
-    if (a.w.K == 0) {
+    const Q4Plan plan = q4_plan(int(sizeof(T)), a.M, a.w.K, a.w.N);
+    if (plan.kernel == Q4_EMPTY) {
         k_q4_empty<T><<<148, Q4_THREADS, 0, st>>>(a);
         note_launch();
         DDG_CUDA(cudaGetLastError());
         return DDG_OK;
     }
-    const GvGeom g = gv_geom(a.w.K, a.w.N, GV_R<T>);
-    // The CUDA cores for one row over Z_2^32 (1 x 1024 x 1024 takes 4.2 us there and 5.6 on the tensor cores,
-    // 1 x 8192 x 8192 18.7 and 22.8), for one over Z_2^64 (twice the limb products) up to 4096 x 4096 (10.5 and
-    // 10.7; 4096 x 8192 18.2 and 16.6), for two of half that (2 x 2048 x 2048 5.9 and 6.7 over Z_2^32, 7.8 and 7.8
-    // over Z_2^64; 2 x 4096 x 4096 10.7 and 9.2).
-    const uint64_t macs = uint64_t(a.M) * uint64_t(a.w.K) * uint64_t(a.w.N);
-    const uint64_t most = a.M == 2 ? 1u << 26 : sizeof(T) == 8 ? 1u << 27 : ~0ull;
-    if (a.M <= 2 && macs * sizeof(T) <= most && gv_smem<T>(g, a.M) <= GV_SMEM_MAX)
-        return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
-    // The tile of least estimated time.  Wide tiles expand the weights fewer times
-    // and split x for more outputs, narrow ones spread a small product over more
-    // SMs: 256 x 1024 x 512 takes 7.1 us in tiles of 32 rows and 9.0 in tiles of
-    // 64; 256 x 4096 x 8192 takes 92 us in tiles of 64 rows by 128 outputs and 58
-    // by 256.  Stage times (us per 64 k) are fits to such measurements.
+    if (plan.kernel == Q4_GEMV) return a.M == 1 ? launch_gemv<T, 1>(a, st) : launch_gemv<T, 2>(a, st);
+    DDG_CHECK(plan.kernel >= 0, DDG_ERR_ARG, "fc_q4: %d rows of K = %d are too many for one call", a.M, a.w.K);
     constexpr int F = sizeof(T) / 4;
-    struct Tile {
-        int mt, na, kc;
-        double us;
-        int (*launch)(const Q4Args<T> &, cudaStream_t);
-    };
-    static const Tile tiles[] = {{4 / F, 1, 128, 0.22, launch_tc_q4<T, 4 / F, 1>},   {8 / F, 1, 128, 0.24, launch_tc_q4<T, 8 / F, 1>},
-                                 {16 / F, 1, 128, 0.28, launch_tc_q4<T, 16 / F, 1>}, {32 / F, 1, 128, 0.42, launch_tc_q4<T, 32 / F, 1>},
-                                 {64 / F, 1, 64, 0.70, launch_tc_q4<T, 64 / F, 1>},  {64 / F, 2, 64, 0.90, launch_tc_q4<T, 64 / F, 2>}};
-    const Tile *best = nullptr;
-    double least = 0;
-    for (const Tile &t : tiles) {
-        const int64_t ctas = (int64_t(a.w.N) + t.na * TC_BM - 1) / (t.na * TC_BM) * ((int64_t(a.M) + t.mt - 1) / t.mt);
-        const int split = qt_split(t.kc, t.na, a.w.K, ctas);
-        const double rounds = double((ctas * split + 147) / 148);
-        const double us = rounds * (2.0 + t.us * double((a.w.K + 63) / 64) / split);
-        const bool fits = (int64_t(a.w.K) + split - 1) / split <= QT_MAX_K && (int64_t(a.M) + t.mt - 1) / t.mt <= 65535;
-        if (fits && (!best || us < least)) best = &t, least = us;
-    }
-    DDG_CHECK(best, DDG_ERR_ARG, "fc_q4: %d rows of K = %d are too many for one call", a.M, a.w.K);
-    return best->launch(a, st);
+    static_assert(QtShape<T, 4 / F, 1>::KC == Q4_TILE[0].kc && QtShape<T, 8 / F, 1>::KC == Q4_TILE[1].kc &&
+                      QtShape<T, 16 / F, 1>::KC == Q4_TILE[2].kc && QtShape<T, 32 / F, 1>::KC == Q4_TILE[3].kc &&
+                      QtShape<T, 64 / F, 1>::KC == Q4_TILE[4].kc && QtShape<T, 64 / F, 2>::KC == Q4_TILE[5].kc,
+                  "stages of the plan and of the kernels");
+    static int (*const launch[Q4_TILES])(const Q4Args<T> &, int, cudaStream_t) = {
+        launch_tc_q4<T, 4 / F, 1>,  launch_tc_q4<T, 8 / F, 1>,  launch_tc_q4<T, 16 / F, 1>,
+        launch_tc_q4<T, 32 / F, 1>, launch_tc_q4<T, 64 / F, 1>, launch_tc_q4<T, 64 / F, 2>};
+    return launch[plan.kernel](a, plan.split, st);
 }
 template int fc_q4<uint32_t>(const Q4Args<uint32_t> &, cudaStream_t);
 template int fc_q4<uint64_t>(const Q4Args<uint64_t> &, cudaStream_t);

@@ -4,6 +4,7 @@
 // the truncation gates between them are the executors' (graph.cuh).
 #pragma once
 #include "common.cuh"
+#include "q4_plan.cuh"
 
 namespace ddg {
 
@@ -19,8 +20,7 @@ struct Q4 {
 };
 inline uint64_t q4_row_bytes(int K) { return 16ull * ((uint64_t(K) + 31) / 32); }
 constexpr int Q4_STEP_MAX = 4095;
-// what one call covers: a cluster of eight CTAs along K, grid rows of 64 (32 over Z_2^64) rows of x
-constexpr int Q4_MAX_K = 8 * 32768;
+// what one call covers: Q4_MAX_K, and grid rows of 64 (32 over Z_2^64) rows of x
 constexpr int q4_max_rows(int bw) { return 65535 * (2048 / bw); }
 
 // out[m][n] = sign * (x . W)[m][n] + bias[n] + Add[m][n] (bias, Add may be null)

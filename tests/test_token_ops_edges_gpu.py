@@ -89,6 +89,79 @@ def test_stride_of_a_single_row_is_not_used(ddg, cuda, bw, K, N):
     assert ddg.lib().ddg_gemm_status() == 0
 
 
+# every kernel and split of K that the choice (csrc/q4_plan.cuh) can make, by ring width:
+# (tile, CTAs along K) -> (M, K, N); tile -2 is the CUDA-core kernel
+FC_TILES = {
+    32: {(-2, 1): (2, 700, 130), (0, 1): (5, 90, 130), (0, 2): (5, 700, 130), (0, 4): (5, 1030, 130),
+         (0, 8): (5, 132010, 130), (1, 1): (299, 90, 130), (1, 2): (161, 700, 130), (1, 4): (79, 1030, 130),
+         (1, 8): (47, 132010, 130), (2, 1): (33, 700, 5000), (2, 2): (299, 700, 130), (2, 4): (161, 1030, 130),
+         (2, 8): (79, 132010, 130), (3, 1): (65, 700, 5000), (3, 2): (65, 700, 2403), (3, 4): (299, 1030, 130),
+         (3, 8): (161, 132010, 130), (4, 1): (100, 90, 5000), (4, 2): (1501, 700, 130), (4, 4): (601, 700, 130),
+         (4, 8): (601, 132010, 3), (5, 1): (199, 90, 5000)},
+    64: {(-2, 1): (1, 700, 130), (0, 1): (3, 90, 130), (0, 2): (3, 700, 130), (0, 4): (3, 1030, 130),
+         (0, 8): (3, 132010, 130), (1, 1): (161, 90, 130), (1, 2): (79, 700, 130), (1, 4): (47, 1030, 130),
+         (1, 8): (21, 132010, 130), (2, 1): (17, 700, 5000), (2, 2): (161, 700, 130), (2, 4): (79, 1030, 130),
+         (2, 8): (47, 132010, 130), (3, 1): (33, 700, 5000), (3, 2): (33, 700, 2403), (3, 4): (161, 1030, 130),
+         (3, 8): (79, 132010, 130), (4, 1): (1501, 700, 130), (4, 2): (601, 700, 130), (4, 4): (299, 700, 130),
+         (4, 8): (161, 132010, 130), (5, 1): (100, 90, 5000)},
+}
+
+
+@pytest.mark.parametrize("bw,tile", [(bw, tile) for bw in FC_TILES for tile in FC_TILES[bw]])
+def test_fc_q4_every_tile_and_split(ddg, cuda, bw, tile):
+    """rows on 16-byte boundaries (tensor maps) and off them (element copies), against float64 limbs"""
+    import torch
+
+    M, K, N = FC_TILES[bw][tile]
+    g = torch.Generator(device="cuda").manual_seed(M + K + N + bw)
+    dt, group = (torch.int32 if bw == 32 else torch.int64), 96
+    rand = lambda *n: torch.randint(-(1 << (bw - 1)), (1 << (bw - 1)) - 1, n, dtype=dt, device="cuda", generator=g)  # noqa: E731
+    q = torch.randint(0, 256, (N, 16 * ((K + 31) // 32)), device="cuda", generator=g).to(torch.uint8)
+    st = torch.randint(0, 4096, ((K + group - 1) // group, N), device="cuda", generator=g).to(torch.int16)
+    code = torch.stack((q & 15, q >> 4), 2).reshape(N, -1)[:, :K].double() - 8
+    W = code.t() * st.double().repeat_interleave(group, 0)[:K]
+    C, b = rand(M, N), rand(N)
+    w = ddg.Q4Weights(K, N, group, ptr(q), ptr(st), ptr(b))
+    for ldx in ((K + 3) // 4 * 4, K | 1):
+        x = rand(M, ldx)
+        out = torch.zeros(M * N + 64, dtype=dt, device="cuda")
+        torch.cuda.synchronize()
+        ddg.fc_q4_share(bw, 0, M, w, ptr(x), ldx, ptr(C), ptr(out))
+        want = C.long() + b.long()
+        for i in range(bw // 16):  # 2^16 x 2^15 x K < 2^53: exact
+            want = want + (torch.matmul(((x[:, :K].long() >> (16 * i)) & 0xFFFF).double(), W).long() << (16 * i))
+        same, behind = bool(torch.equal(out[:M * N].view(M, N), want.to(dt))), int(out[M * N:].count_nonzero())
+        assert same and behind == 0
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+# (M, K, N) whose CTAs on the tensor cores add up the most k that one may: 32,768
+FC_LONGEST = [(3, 32768, 10300), (40, 32768, 10300), (600, 32768, 9000), (1, 262144, 140), (5, 262144, 130),
+              (90, 262144, 70)]
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("M,K,N", FC_LONGEST)
+def test_fc_q4_sums_beyond_31_bits(ddg, cuda, bw, M, K, N):
+    """Every byte of x 255, so that x is -1, and the two bytes of W + 2^15 up to 253 and 238: a column of byte products
+    reaches 491 x 255 x 32768 = 0.955 x 2^32, beyond a signed accumulator's range."""
+    import torch
+
+    dt = torch.int32 if bw == 32 else torch.int64
+    code = torch.tensor([15, 15, 0, 15, 8], device="cuda").repeat(N // 5 + 1)[:N]
+    step = torch.tensor([4059, 4095, 4095, 4022, 1], device="cuda").repeat(N // 5 + 1)[:N]
+    q = (code * 17).to(torch.uint8).view(N, 1).expand(N, 16 * ((K + 31) // 32)).contiguous()
+    st = step.to(torch.int16).expand((K + 31) // 32, N).contiguous()
+    x = torch.full((M, K), -1, dtype=dt, device="cuda")
+    C = torch.arange(M * N, dtype=dt, device="cuda").view(M, N)
+    out = torch.empty(M, N, dtype=dt, device="cuda")
+    torch.cuda.synchronize()
+    ddg.fc_q4_share(bw, 0, M, ddg.Q4Weights(K, N, 32, ptr(q), ptr(st), None), ptr(x), K, ptr(C), ptr(out))
+    want = (C.long() - K * step * (code - 8)).to(dt)
+    same = bool(torch.equal(out, want))
+    assert same and ddg.lib().ddg_gemm_status() == 0
+
+
 # ---------------------------------------------------------------- linear attention
 
 def test_linattn_longest_table_of_powers(ddg, cuda):
