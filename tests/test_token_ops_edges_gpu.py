@@ -320,3 +320,72 @@ def test_wire_calls_refuse_misaligned_arrays(ddg, synth, cuda, bw, off):
     for party in ps:
         party.close()
     d.close()
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("shape", [(1, 12, 520, 64, 64, 128), (1, 30, 200, 47, 33, 64)])
+def test_linattn_on_wires_with_many_heads(ddg, synth, cuda, bw, shape):
+    """Prompt, a prompt from its state, a token: enough heads that the dealer's words and both parties' shares come from
+    the tensor cores in the chunk and output stages; rows on and off 16-byte boundaries."""
+    import torch
+
+    from tests.test_layers_gpu import Bufs, run_both, wire_host
+
+    L, dt = ddg.lib(), ring_dt(bw)
+    s, one = R.Shape(*shape), R.Shape(*shape[:2], 1, *shape[3:])
+    B, H, T, dk, dv, C = shape
+    rng = np.random.default_rng(bw + T)
+    pow_ = ddg.decay_table(bw, S, np.linspace(0.8, 0.99, H), T)
+    sh, sh1 = ddg.LinattnShape(B, H, T, dk, dv, C, T), ddg.LinattnShape(B, H, 1, dk, dv, C, T)
+    new_x = lambda t: np.round(rng.uniform(-0.5, 0.5, (B, t, s.width)) * (1 << S)).astype(np.int64).view(np.uint64)  # noqa: E731
+    x = [new_x(T), new_x(T), new_x(1)]
+    o0, st0 = R.clear_prompt(s, pow_, x[0], None, S, bw)
+    o1, st1 = R.clear_prompt(s, pow_, x[1], st0, S, bw)
+    o2, st2 = R.clear_step(one, pow_[:, 1], x[2], st1, S, bw)
+    want = [o0, st0, o1, st1, o2, st2]
+
+    up = lambda n: -(-n * bw // 8 // 256) * 256  # noqa: E731
+    kb = sum(up(i.size) for i in x) + 2 * L.ddg_linattn_key_bytes(bw, S, sh, 1) + L.ddg_linattn_step_key_bytes(bw, S, sh1)
+    keys, dpow = [dev_bytes(kb) for _ in range(2)], to_dev(pow_)
+    torch.cuda.synchronize()
+    d = ddg.Dealer(bw, S, 0, 17, synth.weights_blob(synth.quantize_weights(synth.affinity_weights(5), S)))
+    d.bind_keys(ptr(keys[0]), ptr(keys[1]), kb)
+    bufs = [Bufs(bw // 8) for _ in range(3)]
+
+    def walk(h, kind, new, inputs):
+        prompt, step = getattr(L, f"ddg_linattn_{kind}"), getattr(L, f"ddg_linattn_step_{kind}")
+        c, X, outs = ddg.Cursor(), [], []
+        for i, v in enumerate(x):
+            X.append(new(v.size))
+            ddg.check(L.ddg_op_input_keygen(h, c, v.size, X[-1]) if inputs is None
+                      else L.ddg_op_input_eval(h, c, v.size, inputs[i], X[-1]))
+        for call, shp, xi, t in ((prompt, sh, X[0], T), (prompt, sh, X[1], T), (step, sh1, X[2], 1)):
+            o, st = new(B * t * H * dv), new(s.n_state)
+            ddg.check(call(h, c, shp, ptr(dpow), xi, outs[-1] if outs else None, o, st))
+            outs += [o, st]
+        return outs, c.offset
+
+    masks, used = walk(d.h, "keygen", lambda n: bufs[2].mask_wire(ddg, n), None)
+    assert 0 < used <= kb
+    sh0 = [rnd(rng, bw, i.size) for i in x]
+    dev = [[to_dev(i) for i in sh0], [to_dev((R.ring(v, bw).reshape(-1) - a).astype(dt)) for v, a in zip(x, sh0)]]
+    torch.cuda.synchronize()
+    ps = [ddg.Party(p, bw, S, 0) for p in (0, 1)]
+    for p, k in zip(ps, keys):
+        p.bind_keys(ptr(k), kb)
+    ddg.pair_local(ps[0], ps[1])
+    got = [None, None]
+
+    def side(p):
+        got[p] = walk(ps[p].h, "eval", lambda n: bufs[p].wire(ddg, n), [ptr(i) for i in dev[p]])
+
+    run_both(lambda: side(0), lambda: side(1))
+    for i, (w, mask) in enumerate(zip(want, masks)):
+        r = wire_host(mask.d_mask, mask.n, dt)
+        for p in (0, 1):
+            v = wire_host(got[p][0][i].d_value, mask.n, dt)
+            assert np.array_equal((v - r).astype(dt), R.ring(w, bw).reshape(-1)), (i, p)
+    assert got[0][1] == got[1][1] == used
+    for p in ps:
+        p.close()
+    d.close()
