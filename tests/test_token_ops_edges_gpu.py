@@ -389,3 +389,77 @@ def test_linattn_on_wires_with_many_heads(ddg, synth, cuda, bw, shape):
     for p in ps:
         p.close()
     d.close()
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+def test_share_calls_of_two_threads_and_two_graphs_at_once(ddg, cuda, bw):
+    """Two host threads on two streams, then two captured graphs replayed at the same time: no call keeps anything that
+    the other one uses."""
+    import threading
+
+    import torch
+
+    M, K, N, T, H = 33, 700, 2403, 300, 20
+    rng = np.random.default_rng(bw)
+    code, step = rng.integers(0, 16, (K, N), dtype=np.uint8), rng.integers(0, 4096, ((K + 31) // 32, N)).astype(np.uint16)
+    W = R.q4_weights(code, step, 32).view(np.uint64)
+    dq, ds = to_dev(R.q4_pack(code)), to_dev(step)
+    s, sh = R.Shape(1, H, T, 48, 96, 100), ddg.LinattnShape(1, H, T, 48, 96, 100, T)
+    w = ddg.Q4Weights(K, N, 32, ptr(dq), ptr(ds), None)
+
+    class Side:
+        def __init__(self):
+            self.st = torch.cuda.Stream()
+            X, C = rnd(rng, bw, M, K), rnd(rng, bw, M, N)
+            x, rx, kd, rkd, z = (rnd(rng, bw, *n) for n in ((1, T, s.width), (1, T, s.width), (s.n_decayed,),
+                                                            (s.n_decayed,), (s.n_ps,)))
+            self.want = (R.ring(R.mm(X, W) + C, bw).reshape(-1), R.ring(R.chunk_share(s, 0, x, rx, kd, rkd) + z, bw))
+            self.d = [to_dev(i) for i in (X, C, x, rx, kd, rkd, z)]
+            self.out = [dev_bytes(i.nbytes) for i in self.want]
+
+        def call(self):
+            X, C, x, rx, kd, rkd, z = (ptr(i) for i in self.d)
+            ddg.fc_q4_share(bw, 0, M, w, X, K, C, ptr(self.out[0]), self.st.cuda_stream)
+            ddg.linattn_chunk_share(bw, 0, sh, s.width, x, rx, kd, rkd, z, ptr(self.out[1]), self.st.cuda_stream)
+
+        def check(self):
+            for o, v in zip(self.out, self.want):
+                assert np.array_equal(from_dev(o, v.dtype, v.size), v)
+                o.zero_()
+            torch.cuda.synchronize()
+
+    sides, errs = [Side(), Side()], []
+    torch.cuda.synchronize()
+
+    def run(side):
+        try:
+            for _ in range(20):
+                side.call()
+        except Exception as e:  # raised below
+            errs.append(e)
+
+    ts = [threading.Thread(target=run, args=(i,)) for i in sides]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join(timeout=60)
+    assert not errs
+    torch.cuda.synchronize()
+    for side in sides:
+        side.check()
+    graphs = []
+    for side in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side.st):
+            side.call()
+    for side in sides:  # capturing ran nothing
+        assert all(int(o.count_nonzero()) == 0 for o in side.out)
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, side in zip(graphs, sides):
+            with torch.cuda.stream(side.st):
+                g.replay()
+    torch.cuda.synchronize()
+    for side in sides:
+        side.check()
+    assert ddg.lib().ddg_gemm_status() == 0
