@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(LA_THREADS)
 // chunk is read once per LC_OT outputs, against a table of decays in shared
 // memory.  The sums cannot be chained from chunk to chunk, because each S_c is
 // floored from exact terms.
-constexpr int LC_OT = 8, LC_SLICE = 4 * LA_THREADS;  // slice: vectors per thread
+constexpr int LC_OT = 8, LC_SLICE = 4 * LA_THREADS;  // slice: vectors per block, four a thread
 
 template <typename T, int V>
 __global__ void __launch_bounds__(LA_THREADS, 3)

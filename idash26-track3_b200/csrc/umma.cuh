@@ -145,14 +145,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&v)[8])
                  : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&v)[4])
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                 : "r"(taddr)
-                 : "memory");
-}
-
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // the four byte planes of four consecutive 32-bit words: plane q holds byte q of e0..e3
@@ -181,14 +173,11 @@ __device__ __forceinline__ void store_planes(uint8_t *base, uint32_t plane_bytes
     }
 }
 
-// asynchronous copy of `bytes` of N bytes (the rest zeros) to shared memory
+// asynchronous copy of `bytes` of N (4 or 8) bytes, the rest zeros, to shared memory
 template <int N>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void *src, int bytes)
 {
-    if constexpr (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
