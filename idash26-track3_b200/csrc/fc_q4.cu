@@ -24,12 +24,19 @@
 // MMAs, the others expand codes and split x.  The sums of a split K meet in the
 // cluster's shared memory.
 //
-// Measured on one B200 (graph replays, launch included): CUDA cores, 1 x 376 x
-// 1024 4.1 us, 1 x 4096 x 4096 7.6 us and 1 x 4096 x 8192 11.2 us (1.5 TB/s of codes;
-// the limb products' issue); tensor cores, 256 x 1024 x 512 7.1 us,
-// 16 x 4096 x 8192 15.0 us (16.8 MB of codes, 1.1 TB/s: bound by the expansion
-// in its sixteen warps), 2048 x 4096 x 4096 230 us (0.30 P ring flop/s, 1.2 P byte
-// products/s: tensor pipe 62 % busy, bound by shared memory).
+// Measured on one B200 (graph replays, launch included, weights from memory).
+// CUDA cores: 1 x 376 x 1024 4.0 us, 1 x 4096 x 4096 9.3 us and 1 x 4096 x 8192
+// 13.0 us (1.3 TB/s of codes), 7.7 and 10.7 with the weights in L2; over Z_2^64
+// 1 x 4096 x 4096 12.7.  Bound by latency: a scheduler issues in 0.34 to 0.38 of
+// its cycles, 21 % of the warps are there, and a warp waits 2.8 of its 9 cycles an
+// instruction for memory, 0.7 to 1.1 at barriers, 1 for shared memory; each is
+// one chain of the split of x and its segments, with one segment in flight.
+// Tensor cores: 256 x 1024 x 512 7.1 us; 16 x 4096 x 8192 18.0 us (16.8 MB of
+// codes, 0.9 TB/s; 14.5 in L2), bound by the hand-off of a stage from copy to
+// expansion to MMA in one CTA an SM (issue 0.40, tensor pipe 13 %, 4.1 of 11
+// cycles an instruction waiting for memory or tensor memory); 2048 x 4096 x 4096
+// 229 us (0.30 P ring flop/s, 1.2 P byte products/s: tensor pipe 62 % busy, bound
+// by shared memory), over Z_2^64 468 us.
 #include <type_traits>
 
 #include "tma.cuh"

@@ -207,9 +207,10 @@ __global__ void __launch_bounds__(LA_THREADS, 3)
 // memory, whose bandwidth the planes and the MMAs' own reads take), split the
 // present one into planes and hand the stage over by mbarrier; there is no
 // CTA-wide barrier in the loop, and loads run on across tiles.  What bounds
-// these kernels is the loads' latency against what the registers hold in flight,
-// so every load covers whole 128-byte lines and whole tiles take loads without
-// bounds.
+// these kernels is the loads' latency against what the registers hold in flight
+// (the largest wait of every warp, 2.4 of 8 cycles an instruction, over Z_2^64 6.2
+// of 11.5; issue 0.47 and 0.32, tensor pipe 16 to 23 %, DRAM a third), so every load
+// covers whole 128-byte lines and whole tiles take loads without bounds.
 constexpr int LT_WARPS = 8, LT_THREADS = LT_WARPS * 32;
 
 template <typename T>
@@ -834,8 +835,11 @@ __global__ void __launch_bounds__(LA_THREADS)
 // the new state written once (4 words moved and 5 multiply-adds per entry, so
 // bound by memory); q . S comes out of the same pass, summed over the thread
 // rows in shared memory.  Two rows ahead and four blocks an SM: 1024 heads x 128 x
-// 128 in 50 us (5.3 TB/s), 512 x 64 x 128 over Z_2^64 in 31 us; four rows and three
-// blocks took 54 and 39, one wave of blocks that loop over heads 73 and 47.
+// 128 in 50 us (5.3 TB/s), 512 x 64 x 128 over Z_2^64 in 31 us (4.3 TB/s: as many
+// blocks with half the bytes each, so what a block does once, its first loads and the
+// sum over its rows, weighs twice; barriers take 2 of 16 cycles an instruction there,
+// 1.3 of 22 here); four rows and three blocks took 54 and 39, one wave of blocks that
+// loop over heads 73 and 47.
 template <typename T, int V>
 __global__ void __launch_bounds__(LA_THREADS, 4)
     k_la_step(const LaShape s, const __grid_constant__ LaStepArgs<T> a, int cx, int slabs)
@@ -978,6 +982,8 @@ inline unsigned la_tile_grid(int64_t tiles) { return unsigned(tiles < 2 * 148 ? 
 // 10.0 / 10.2 / 17.8 against 17.3 / 17.4 / 17.5 (24 heads: 16.5 and 17.3), over Z_2^64
 // 22.9 / 23.1 / 41.6 against 23.2 / 23.2 / 23.4, and for 16 heads x 32 tokens there
 // 13.0 against 13.9; 16 heads x 138 tokens x 47 (304 tiles) chunk stage 11.2 and 19.7.
+// Tiles are counted without their K, so short prompts leave the CUDA cores early: the
+// chunk stage of 32 heads x 8 tokens over Z_2^64 takes 15.5 where 11.6 is possible.
 static bool ls_fits(const LaShape &s, int64_t tiles_full, int64_t tiles_last, int64_t most)
 {
     return s.bh() * ((s.chunks() - 1) * tiles_full + tiles_last) <= most;

@@ -72,19 +72,24 @@ struct Q4Plan {
 inline Q4Plan q4_plan(int elem, int M, int K, int N)
 {
     if (K == 0) return {Q4_EMPTY, 1};
-    // The CUDA cores for one row over Z_2^32 (1 x 1024 x 1024 takes 4.2 us there and 5.6 on the tensor cores,
-    // 1 x 8192 x 8192 18.7 and 22.8), for one over Z_2^64 (twice the limb products) up to 4096 x 4096 (10.5 and
-    // 10.7; 4096 x 8192 18.2 and 16.6), for two of half that (2 x 2048 x 2048 5.9 and 6.7 over Z_2^32, 7.8 and 7.8
-    // over Z_2^64; 2 x 4096 x 4096 10.7 and 9.2).
+    // The CUDA cores for one row over Z_2^32, for one over Z_2^64 (twice the limb products) up to 4096 x 4096, for two
+    // of half that.  In us with the weights in L2 (from memory), CUDA cores against tensor cores: over Z_2^32
+    // 1 x 1024 x 1024 4.1 (4.3) against 5.4 (5.4), 1 x 8192 x 8192 18.0 (21.6) against 22.2 (26.0), 2 x 2048 x 2048
+    // 5.7 (7.1) against 6.8 (7.8), 2 x 4096 x 4096 10.5 (12.3) against 9.2 (10.9); over Z_2^64 1 x 4096 x 4096 10.6
+    // (12.7) against 10.7 (11.7), 1 x 4096 x 8192 16.7 (19.9) against 15.9 (17.0), 2 x 2048 x 2048 7.6 (8.6) against
+    // 7.8 (8.7).  The work alone decides, so one row of a wide, short layer over Z_2^64 is on the slower side:
+    // 1 x 1024 x 16384 11.2 (14.4) against 9.7 (10.9).
     const uint64_t macs = uint64_t(M) * uint64_t(K) * uint64_t(N);
     const uint64_t most = M == 2 ? 1u << 26 : elem == 8 ? 1u << 27 : ~0ull;
     if (M <= 2 && macs * unsigned(elem) <= most && gv_smem(gv_geom(K, N, gv_outputs(elem)), M, elem) <= GV_SMEM_MAX)
         return {Q4_GEMV, 1};
     // The tile of least estimated time.  Wide tiles expand the weights fewer times
     // and split x for more outputs, narrow ones spread a small product over more
-    // SMs: 256 x 1024 x 512 takes 7.1 us in tiles of 32 rows and 9.0 in tiles of
-    // 64; 256 x 4096 x 8192 takes 92 us in tiles of 64 rows by 128 outputs and 58
-    // by 256.  Stage times (us per 64 k) are fits to such measurements.
+    // SMs: 256 x 1024 x 512 takes 7.4 us in tiles of 32 rows and 9.6 in tiles of
+    // 64; 256 x 4096 x 8192 takes 93 us in tiles of 64 rows by 128 outputs and 58
+    // by 256.  Stage times (us per 64 k) are fits to such measurements, with rows of x
+    // on 16-byte boundaries; off them the copies of x add to every stage (256 x
+    // 1004 x 4096 takes 19.7 us and 256 x 1003 x 4096 26.9).
     Q4Plan best = {Q4_NONE, 1};
     double least = 0;
     for (int i = 0; i < Q4_TILES; i++) {
