@@ -15,6 +15,14 @@ def rnd(rng, bw, *shape):
     return rng.integers(0, np.iinfo(dt).max, size=shape, dtype=dt, endpoint=True)
 
 
+@pytest.fixture
+def room(cuda):
+    """the allocator's cache of a large test, given back for the library's own allocations of the next one"""
+    yield
+    cuda.cuda.synchronize()
+    cuda.cuda.empty_cache()
+
+
 # ---------------------------------------------------------------- 4-bit weights
 
 LONGEST_GROUP = (1 << 31) - 32
@@ -41,7 +49,7 @@ def test_one_step_per_output_as_a_group_beyond_K(ddg, cuda, K, group):
             assert np.array_equal(from_dev(out, ring_dt(bw), M * N).reshape(M, N), R.ring(R.mm(X, W) + C, bw))
 
 
-def test_q4_quantize_of_the_longest_column(ddg, cuda):
+def test_q4_quantize_of_the_longest_column(ddg, cuda, room):
     """K = 2^31 - 1: the row's last byte, half of it padding, and the last group's step are written."""
     import torch
 
@@ -142,7 +150,7 @@ FC_LONGEST = [(3, 32768, 10300), (40, 32768, 10300), (600, 32768, 9000), (1, 262
 
 @pytest.mark.parametrize("bw", [32, 64])
 @pytest.mark.parametrize("M,K,N", FC_LONGEST)
-def test_fc_q4_sums_beyond_31_bits(ddg, cuda, bw, M, K, N):
+def test_fc_q4_sums_beyond_31_bits(ddg, cuda, room, bw, M, K, N):
     """Every byte of x 255, so that x is -1, and the two bytes of W + 2^15 up to 253 and 238: a column of byte products
     reaches 491 x 255 x 32768 = 0.955 x 2^32, beyond a signed accumulator's range."""
     import torch
@@ -164,7 +172,7 @@ def test_fc_q4_sums_beyond_31_bits(ddg, cuda, bw, M, K, N):
 
 # ---------------------------------------------------------------- linear attention
 
-def test_linattn_longest_table_of_powers(ddg, cuda):
+def test_linattn_longest_table_of_powers(ddg, cuda, room):
     """pow_n = 2^31 - 1: the second head's powers start 2^31 elements into the table."""
     import torch
 
@@ -462,4 +470,135 @@ def test_share_calls_of_two_threads_and_two_graphs_at_once(ddg, cuda, bw):
     torch.cuda.synchronize()
     for side in sides:
         side.check()
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+# ---------------------------------------------------------------- long calls
+
+def big(bw, *n, seed=0):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(n))
+    dt = torch.int32 if bw == 32 else torch.int64
+    return torch.randint(-(1 << 31), (1 << 31) - 1, n, dtype=dt, device="cuda", generator=g)
+
+
+def host(t):
+    return t.cpu().numpy().astype(np.int64).view(np.uint64)
+
+
+@pytest.mark.parametrize("bw", [32, 64])
+@pytest.mark.parametrize("T,C", [(2048, 1), (262144, 128), (262100, 128)])
+def test_linattn_most_chunks(ddg, cuda, bw, T, C):
+    """2048 chunks: the longest prompt of one call, and as many chunks of one token"""
+    rng = np.random.default_rng(T + C + bw)
+    B, H, dk, dv, nc = 1, 2, 2, 3, 2048
+    s, sh = R.Shape(B, H, T, dk, dv, C), ddg.LinattnShape(B, H, T, dk, dv, C, T)
+    pow_, x, rx = rnd(rng, bw, H, T + 1), rnd(rng, bw, B, T, s.width), rnd(rng, bw, B, T, s.width)
+    kd, rkd, ps, rps = (rnd(rng, bw, n) for n in (s.n_decayed, s.n_decayed, s.n_ps, s.n_ps))
+    s0, rs0, z, z2 = (rnd(rng, bw, n) for n in (s.n_state, s.n_state, s.n_ps, T * H * dv))
+    d = [to_dev(i) for i in (pow_, x, rx, kd, rkd, ps, rps, s0, rs0, z, z2)]
+    dp, dx, drx, dkd, drkd, dps, drps, ds0, drs0, dz, dz2 = (ptr(i) for i in d)
+    o1, o2 = dev_bytes(2 * s.n_decayed * bw // 8), dev_bytes(s.n_ps * bw // 8)
+    ddg.linattn_decay(bw, sh, s.width, dp, dx, ptr(o1))
+    ddg.linattn_carry(bw, sh, dp, dps, ds0, ptr(o2))
+    ddg.linattn_chunk_share(bw, 0, sh, s.width, dx, drx, dkd, drkd, dz, dz)
+    ddg.linattn_output_share(bw, 1, sh, s.width, dx, drx, dkd, drkd, dps, drps, ds0, drs0, dz2, dz2)
+    assert np.array_equal(from_dev(o1, ring_dt(bw), 2 * s.n_decayed), R.ring(R.decay(s, pow_, x), bw))
+    assert np.array_equal(from_dev(d[9], z.dtype, z.size), R.ring(R.chunk_share(s, 0, x, rx, kd, rkd) + z, bw))
+    assert np.array_equal(from_dev(d[10], z.dtype, z2.size),
+                          R.ring(R.output_share(s, 1, x, rx, kd, rkd, ps, rps, s0, rs0) + z2, bw))
+    # the carry: every chunk's state as one product with the decays from chunk to chunk
+    got, p64, U = from_dev(o2, ring_dt(bw), s.n_ps), pow_.astype(np.uint64), np.uint64
+    full, st = s.split_ps(ps)
+    ends = np.array([e for _, e in s.spans])
+    gap = ends[:, None] - ends[None, :]
+    for h in range(H):
+        w = np.where(gap >= 0, p64[h][np.maximum(gap, 0)], U(0))
+        want = R.mm(w, st[:, 0, h].reshape(nc, -1))
+        want += p64[h][ends][:, None] * s0.astype(np.uint64).reshape(H, -1)[h][None, :]
+        assert np.array_equal(got[s.n_scores:].reshape(nc, H, -1)[:, h], R.ring(want, bw))
+    i, j = np.tril_indices(C)
+    gaps = np.concatenate([(i - j)[:m * (m + 1) // 2] for m in np.diff(np.concatenate([[0], ends]))])
+    want = ps[:s.n_scores].astype(np.uint64).reshape(H, -1) * p64[:, gaps]
+    assert np.array_equal(got[:s.n_scores].reshape(H, -1), R.ring(want, bw))
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+def test_fc_q4_offsets_beyond_32_bits(ddg, cuda, room):
+    """4.9 GB of codes under one row; 2.9 G outputs, in place"""
+    import torch
+
+    for M, K, N in ((1, 16384, 600001), (700001, 64, 4100)):
+        q = torch.randint(0, 256, (N, K // 2), device="cuda", dtype=torch.uint8)
+        st = torch.randint(0, 4096, (K // 32, N), device="cuda", dtype=torch.int16)
+        x, C, m, n = big(32, M, K), big(32, M, N), min(M, 300), min(N, 300)
+        was = C[-m:, -n:].clone()
+        torch.cuda.synchronize()
+        ddg.fc_q4_share(32, 0, M, ddg.Q4Weights(K, N, 32, ptr(q), ptr(st), None), ptr(x), K, ptr(C), ptr(C))
+        code = torch.stack((q[-n:] & 15, q[-n:] >> 4), 2).reshape(n, K).double() - 8
+        W, want = code.t() * st[:, -n:].double().repeat_interleave(32, 0), was.long()
+        for i in range(2):  # 2^16 x 2^15 x K < 2^53: exact
+            want = want + (torch.matmul(((x[-m:].long() >> (16 * i)) & 0xFFFF).double(), W).long() << (16 * i))
+        same = bool(torch.equal(C[-m:, -n:], want.to(torch.int32)))
+        assert same
+        del q, st, x, C
+        torch.cuda.empty_cache()
+    assert ddg.lib().ddg_gemm_status() == 0
+
+
+def test_linattn_offsets_beyond_32_bits(ddg, cuda, room):
+    """128 x 16 heads x 16,384 tokens: 3.2 G elements of q|k|v, 2.4 G of scores and states; the last head's last chunk"""
+    import torch
+
+    B, H, T, dk, dv, C = 128, 16, 16384, 32, 32, 128
+    s = R.Shape(1, 1, C, dk, dv, C)  # what is compared
+    sh = ddg.LinattnShape(B, H, T, dk, dv, C, T)
+    size = ddg.linattn_sizes(sh)
+    assert size["qkv"] > 1 << 31 and size["ps"] > 1 << 31
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 90 GB of device memory")
+    width, tri, bh = H * 96, (T // C) * (C * (C + 1) // 2), B * H
+    pow_ = rnd(np.random.default_rng(2), 32, H, T + 1)
+    dp, x, rx = to_dev(pow_), big(32, B * T, width), big(32, B * T, width, seed=1)
+    kd, rkd = big(32, 2, bh, T, dk), big(32, 2, bh, T, dk, seed=1)
+    ps, rps, z = big(32, size["ps"]), big(32, size["ps"], seed=1), big(32, size["ps"], seed=2)
+
+    def last(t):  # [the last head's last chunk of scores | its state, and the one before]
+        a, n = bh * tri, bh * dk * dv
+        return [host(t[a - C * (C + 1) // 2:a])] + [host(t[a + c * n - dk * dv:a + c * n]) for c in (T // C, T // C - 1)]
+
+    def tail(t):  # q, k, v of that chunk, as one head's rows
+        r = host(t[-C:])
+        return np.concatenate([r[:, (o + 1) * H * 32 - 32:(o + 1) * H * 32] for o in range(3)], 1)[None]
+
+    lx, lrx, (p, s_end, s_in), (rp, rs_end, rs_in), z0 = tail(x), tail(rx), last(ps), last(rps), last(z)
+    lkd, lrkd = (host(t[:, -1, -C:]) for t in (kd, rkd))
+    torch.cuda.synchronize()
+    ddg.linattn_chunk_share(32, 0, sh, width, ptr(x), ptr(rx), ptr(kd[1]), ptr(rkd[1]), ptr(z), ptr(z))
+    got, want = last(z), R.chunk_share(s, 0, lx, lrx, lkd[1], lrkd[1])
+    assert np.array_equal(R.ring(got[0], 32), R.ring(want[:s.n_scores] + z0[0], 32))
+    assert np.array_equal(R.ring(got[1], 32), R.ring(want[s.n_scores:] + z0[1], 32))
+    ddg.linattn_carry(32, sh, ptr(dp), ptr(ps), None, ptr(z))
+    got = last(z)
+    i, j = np.tril_indices(C)
+    lam = pow_[-1].astype(np.uint64)
+    assert np.array_equal(R.ring(got[0], 32), R.ring(p * lam[i - j], 32))
+    n, nc = bh * dk * dv, T // C
+    st = np.stack([host(ps[bh * tri + (c + 1) * n - dk * dv:bh * tri + (c + 1) * n]) for c in range(nc)])
+    assert np.array_equal(R.ring(got[1], 32), R.ring(R.mm(lam[T - C * (1 + np.arange(nc))][None], st)[0], 32))
+    out = big(32, B * T, H * dv, seed=3)
+    o0 = host(out[-C:, -dv:])
+    torch.cuda.synchronize()
+    ddg.linattn_output_share(32, 0, sh, width, ptr(x), ptr(rx), ptr(kd), ptr(rkd), ptr(ps), ptr(rps), None, None,
+                             ptr(out), ptr(out))
+    join = lambda a, b: np.concatenate([a, b])  # noqa: E731
+    want = R.output_share(s, 0, lx, lrx, lkd[0], lrkd[0], join(p, s_in), join(rp, rs_in), s_in, rs_in)
+    assert np.array_equal(R.ring(host(out[-C:, -dv:]), 32).reshape(-1), R.ring(want + o0.reshape(-1), 32))
+    ddg.linattn_decay(32, sh, width, ptr(dp), ptr(x), ptr(kd))
+    w2 = lx.copy()
+    w2[0, :, :dk] *= lam[1:C + 1, None]
+    w2[0, :, dk:2 * dk] *= lam[C - 1::-1, None][:C]
+    for half in (0, 1):
+        assert np.array_equal(R.ring(host(kd[half, -1, -C:]), 32), R.ring(w2[0, :, half * dk:(half + 1) * dk], 32))
     assert ddg.lib().ddg_gemm_status() == 0
