@@ -551,7 +551,8 @@ int ddg_fc_q4_share(int bw, int party, int M, const ddg_q4_weights *w, const voi
 typedef struct ddg_linattn_shape {
     int batch, heads, tokens, dk, dv, chunk, pow_n;
 } ddg_linattn_shape;
-/* host: h_pow (heads x (n + 1) ring elements) = round(lambda^i * 2^scale), h_lambda in [0, 1] */
+/* host: h_pow (heads x (n + 1) ring elements) = round(lambda^i * 2^scale), h_lambda in [0, 1]; the powers are
+ * repeated products in double precision, within i * 2^-53 of lambda^i relative to it before the rounding */
 int ddg_decay_table(int bw, int scale, int heads, int n, const double *h_lambda, void *h_pow);
 /* array sizes in ring elements: out6 = {qkv at the least ld, qkd, ps, state, step output, out} */
 int ddg_linattn_sizes(const ddg_linattn_shape *shape, int64_t *out6);
