@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(LA_THREADS)
         for (int e = threadIdx.x; e < 2 * half; e += LA_THREADS) {
             const bool key = e >= half;
             const int r = key ? e - half : e, h = r / dkv, d = r - h * dkv;
-            const T p = __ldg(pow + s.pow_at(h) + (key ? back : i + 1));
+            const T p = __ldg(pow + s.pow_at(uint32_t(h)) + (key ? back : i + 1));
             Pack<T, V> v = row[e];
 #pragma unroll
             for (int j = 0; j < V; j++) v.e[j] *= p;
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(LA_THREADS, 4)
         qs[i] = __ldg(a.qkv + oq + i), ks[i] = __ldg(a.qkv + ok + i);
         rq[i] = a.qkv_ms ? __ldg(a.qkv_ms + oq + i) : T(0), rk[i] = a.qkv_ms ? __ldg(a.qkv_ms + ok + i) : T(0);
     }
-    const T lam = a.lam * __ldg(a.pow + s.pow_at(h) + 1);
+    const T lam = a.lam * __ldg(a.pow + s.pow_at(uint32_t(h)) + 1);
     __syncthreads();
     for (int i0 = y0; i0 < s.dk; i0 += U * ry) {
 #pragma unroll
@@ -931,7 +931,7 @@ __global__ void __launch_bounds__(LA_THREADS)
     {
         const int64_t bh = e / s.dv, b = bh / s.H, h = bh % s.H;
         const int64_t ov = b * a.ld + 2 * int64_t(s.H) * s.dk + h * s.dv + e % s.dv;
-        T right = a.p0 * a.qkv[ov], acc = a.lam * a.pow[s.pow_at(h) + 1] * a.yw[e];
+        T right = a.p0 * a.qkv[ov], acc = a.lam * a.pow[s.pow_at(uint32_t(h)) + 1] * a.yw[e];
         if (a.qkv_ms) right -= a.qkv_ms[ov], acc -= a.yw_ms[ny + bh] * a.qkv[ov];
         a.out[e] = acc + a.yw[ny + bh] * right + a.z[e];
     }

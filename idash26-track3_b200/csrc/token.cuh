@@ -62,7 +62,8 @@ struct LaShape {
         const int64_t r = T % C;
         return tri_at(T / C) + r * (r + 1) / 2;
     }
-    __host__ __device__ int64_t pow_at(int64_t h) const { return h * (int64_t(pn) + 1); }  // pn may be the largest int
+    // (pn may be the largest int; one 32 x 32-bit multiply)
+    __host__ __device__ int64_t pow_at(uint32_t h) const { return int64_t(uint64_t(h) * (uint32_t(pn) + 1u)); }
     __host__ __device__ int64_t width() const { return int64_t(H) * (2 * int64_t(dk) + dv); }
     __host__ __device__ int64_t n_qkv() const { return int64_t(B) * T * width(); }
     __host__ __device__ int64_t n_decayed() const { return bh() * T * dk; }  // of each of Qd, Kd
